@@ -16,7 +16,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "libfa2_b200.so")
-SOURCES = ["api.cu", "fwd_sm100.cu", "fwd256_sm100.cu", "fwd_combine.cu", "bwd_sm100.cu", "bwd256_sm100.cu"]
+SOURCES = ["api.cu", "fwd_sm100.cu", "fwd256_sm100.cu", "fwd_combine.cu", "bwd_sm100.cu", "bwd256_sm100.cu",
+           "fwd_scored64_sm100.cu", "fwd_scored128_sm100.cu", "fwd_scored256_sm100.cu",
+           "bwd_scored64_sm100.cu", "bwd_scored128_sm100.cu", "bwd_scored256_sm100.cu", "document_layout.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
@@ -36,6 +38,7 @@ def _newest_input() -> float:
     paths = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     paths.append(os.path.join(HERE, "..", "include", "fa2_b200.h"))
     paths.append(os.path.join(HERE, "..", "include", "fa2_b200_debug.h"))
+    paths.append(os.path.join(HERE, "..", "include", "fa2_b200_lm.h"))
     paths.append(os.path.abspath(__file__))
     return max(os.path.getmtime(p) for p in paths)
 

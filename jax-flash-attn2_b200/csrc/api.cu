@@ -16,9 +16,12 @@
 
 #include "../../include/fa2_b200.h"
 #include "../../include/fa2_b200_debug.h"
+#include "../../include/fa2_b200_lm.h"
 #include "bwd_launch.cuh"
 #include "fwd_launch.cuh"
 #include "launch_util.cuh"
+#include "lm_launch.cuh"
+#include "score_mod.cuh"
 
 namespace fa2 {
 namespace {
@@ -327,6 +330,69 @@ bool can_pack_heads(const fa2_problem& p) {
   return p.seqlen_q == 1 && group > 1 && group <= 128 && !(p.dropout_p > 0.f);
 }
 
+// Sizes and parts of a document layout (int32): token bounds [B][S] twice, tile bounds [B][ceil(S/128)] twice.
+size_t document_layout_ints(int64_t batch, int64_t seqlen) {
+  return static_cast<size_t>(batch) * (2 * static_cast<size_t>(seqlen) + 2 * ((static_cast<size_t>(seqlen) + 127) / 128));
+}
+
+constexpr float kMinSoftcap = 1.f / 1024.f, kMaxSoftcap = 1024.f;
+
+int check_softcap(float cap) {
+  if (cap != 0.f && !(cap >= kMinSoftcap && cap <= kMaxSoftcap))
+    return fail(FA2_ERR_INVALID_ARG, "softcap must be 0 (none) or in [2^-10, 1024]");
+  return FA2_OK;
+}
+
+// Checks the score changes of a call and fills the kernels' record; `mode` receives kModCap | kModSlope.
+int make_score_mod(ScoreModDev* out, int* mode, const fa2_score_mod& m, const fa2_problem& p) {
+  std::memset(out, 0, sizeof(*out));
+  const int rc = check_softcap(m.softcap);
+  if (rc) return rc;
+  if (!(p.softmax_scale >= 1e-30f))
+    return fail(FA2_ERR_INVALID_ARG, "softmax_scale must be positive in attention with changed scores");
+  if (p.dropout_p > 0.f) return fail(FA2_ERR_UNSUPPORTED, "dropout is not supported in attention with changed scores");
+  if (m.prefix_lens && !p.causal) return fail(FA2_ERR_INVALID_ARG, "prefix_lens needs causal masking");
+  if (m.document_layout && p.seqlen_q != p.seqlen_k)
+    return fail(FA2_ERR_INVALID_ARG, "documents require seqlen_q == seqlen_k");
+  if ((reinterpret_cast<uintptr_t>(m.alibi_slopes) | reinterpret_cast<uintptr_t>(m.prefix_lens) |
+       reinterpret_cast<uintptr_t>(m.document_layout)) & 3)
+    return fail(FA2_ERR_INVALID_ARG, "alibi_slopes, prefix_lens and document_layout must be 4-byte aligned");
+  *mode = 0;
+  if (m.softcap > 0.f) {
+    *mode |= kModCap;
+    out->cap2 = static_cast<float>(m.softcap * 1.4426950408889634);
+    out->arg2 = static_cast<float>(2.0 * p.softmax_scale * 1.4426950408889634 / m.softcap);
+    if (!std::isfinite(out->arg2)) return fail(FA2_ERR_INVALID_ARG, "softmax_scale / softcap overflows");
+  }
+  if (m.alibi_slopes) *mode |= kModSlope;
+  out->slopes = m.alibi_slopes;
+  out->prefix_lens = m.prefix_lens;
+  out->causal = p.causal != 0;
+  if (m.document_layout) {
+    const size_t tokens = static_cast<size_t>(p.batch) * p.seqlen_q;
+    const size_t tiles = static_cast<size_t>(p.batch) * ((static_cast<size_t>(p.seqlen_q) + 127) / 128);
+    out->tok_lo = m.document_layout;
+    out->tok_hi = out->tok_lo + tokens;
+    out->tile_lo = out->tok_hi + tokens;
+    out->tile_hi = out->tile_lo + tiles;
+  }
+  return FA2_OK;
+}
+
+cudaError_t launch_fwd_scored(const FwdLaunch& a, int mode, cudaStream_t stream) {
+  return a.head_dim == 64    ? launch_fwd_scored64(a, mode, stream)
+         : a.head_dim == 128 ? launch_fwd_scored128(a, mode, stream)
+                             : launch_fwd_scored256(a, mode, stream);
+}
+cudaError_t launch_bwd_scored(const BwdLaunch& a, int mode, cudaStream_t stream) {
+  return a.head_dim == 64    ? launch_bwd_scored64(a, mode, stream)
+         : a.head_dim == 128 ? launch_bwd_scored128(a, mode, stream)
+                             : launch_bwd_scored256(a, mode, stream);
+}
+
+int fwd_impl(const fa2_fwd_params* a, const fa2_score_mod* mod, void* cuda_stream);
+int bwd_impl(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_stream);
+
 }  // namespace
 }  // namespace fa2
 
@@ -356,7 +422,128 @@ int fa2_debug_bwd_stage_events(void* const* events) {
   return FA2_OK;
 }
 
-int fa2_fwd(const fa2_fwd_params* a, void* cuda_stream) {
+int fa2_fwd(const fa2_fwd_params* a, void* cuda_stream) { return fwd_impl(a, nullptr, cuda_stream); }
+
+size_t fa2_fwd_workspace_bytes(const fa2_problem* problem) {
+  if (!problem || check_problem(*problem)) return 0;
+  HeadDim hd;
+  split_head_dim(problem->head_dim, &hd);
+  // whether grouped heads get packed also depends on operands this function does not see
+  // (bias, mask, lengths): report what the larger of the two plans needs
+  size_t need = plan_splits(*problem, hd, false).total;
+  if (can_pack_heads(*problem)) need = std::max(need, plan_splits(*problem, hd, true).total);
+  return need;
+}
+
+size_t fa2_dropout_bits_bytes(const fa2_problem* problem) {
+  if (!problem || check_problem(*problem)) return 0;
+  return dropout_bits_bytes(*problem);
+}
+
+size_t fa2_bwd_workspace_bytes(const fa2_problem* problem) {
+  if (!problem || check_problem(*problem)) return 0;
+  return bwd_workspace(*problem).total;
+}
+
+int fa2_bwd(const fa2_bwd_params* a, void* cuda_stream) { return bwd_impl(a, nullptr, cuda_stream); }
+
+// ---------------------------------------------------------------------------------------------
+// Backward without a caller-provided workspace
+// ---------------------------------------------------------------------------------------------
+namespace {
+// Scratch of the backward (row statistics + fp32 dq accumulator) for callers that cannot hand
+// in device memory of their own. One array per GPU that loads the library, held until exit.
+static __device__ __align__(256) unsigned char g_bwd_static_scratch[FA2_BWD_STATIC_SCRATCH_BYTES];
+
+constexpr int kMaxDevices = 64;
+void* g_static_scratch_ptr[kMaxDevices] = {};
+std::mutex g_static_scratch_mutex;
+
+// Device address of the array on the current device. In host code the array's name is only a
+// handle for the runtime, not an address a kernel could use, so the address is looked up once per
+// device (with that device current) and cached.
+int static_scratch_address(void** out) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return fail(FA2_ERR_CUDA, "cannot identify the current CUDA device");
+  std::lock_guard<std::mutex> lock(g_static_scratch_mutex);
+  if (!g_static_scratch_ptr[dev]) {
+    void* ptr = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&ptr, g_bwd_static_scratch);
+    if (e != cudaSuccess || !ptr)
+      return fail(FA2_ERR_CUDA, "cudaGetSymbolAddress failed for the static scratch: %s",
+                  cudaGetErrorString(e));
+    g_static_scratch_ptr[dev] = ptr;
+  }
+  *out = g_static_scratch_ptr[dev];
+  return FA2_OK;
+}
+}  // namespace
+
+int fa2_bwd_static_scratch(const fa2_bwd_params* a, void* cuda_stream) {
+  if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
+  const int rc = check_problem(a->p);
+  if (rc) return rc;
+  const size_t need = bwd_workspace(a->p).total;
+  if (need > static_cast<size_t>(FA2_BWD_STATIC_SCRATCH_BYTES))
+    return fail(FA2_ERR_WORKSPACE,
+                "this problem needs %zu bytes of scratch; the built-in scratch holds %zu bytes "
+                "(batch * heads_q * ceil(seqlen_q/128)*128 * (head_dim + 2) * 4 must not exceed it); "
+                "use fa2_bwd with a workspace instead",
+                need, static_cast<size_t>(FA2_BWD_STATIC_SCRATCH_BYTES));
+  void* scratch = nullptr;
+  const int rs = static_scratch_address(&scratch);
+  if (rs) return rs;
+  fa2_bwd_params b = *a;
+  b.workspace = scratch;
+  b.workspace_bytes = FA2_BWD_STATIC_SCRATCH_BYTES;
+  return fa2_bwd(&b, cuda_stream);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention with changed scores (fa2_b200_lm.h)
+// ---------------------------------------------------------------------------------------------
+int fa2_lm_version(void) { return FA2_LM_ABI_VERSION; }
+
+int fa2_scored_fwd(const fa2_fwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
+  if (!mod) return fail(FA2_ERR_INVALID_ARG, "mod is null");
+  return fwd_impl(a, mod, cuda_stream);
+}
+
+int fa2_scored_bwd(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
+  if (!mod) return fail(FA2_ERR_INVALID_ARG, "mod is null");
+  return bwd_impl(a, mod, cuda_stream);
+}
+
+size_t fa2_document_layout_bytes(int32_t batch, int32_t seqlen) {
+  if (batch <= 0 || seqlen <= 0) return 0;
+  return document_layout_ints(batch, seqlen) * sizeof(int32_t);
+}
+
+int fa2_document_layout(const int32_t* document_ids, int64_t stride_b, int32_t batch, int32_t seqlen, int32_t* layout,
+                        size_t layout_bytes, void* cuda_stream) {
+  if (!document_ids || !layout) return fail(FA2_ERR_INVALID_ARG, "document_ids and layout must be non-null");
+  if (batch <= 0 || seqlen <= 0) return fail(FA2_ERR_INVALID_ARG, "batch and seqlen must be positive");
+  if (seqlen > INT_MAX - 8192) return fail(FA2_ERR_UNSUPPORTED, "seqlen must stay below 2^31 - 8192");
+  if (stride_b < 0) return fail(FA2_ERR_INVALID_ARG, "the stride of document_ids must be non-negative");
+  if (reinterpret_cast<uintptr_t>(document_ids) & 3)
+    return fail(FA2_ERR_INVALID_ARG, "document_ids must be 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(layout) & 15) return fail(FA2_ERR_INVALID_ARG, "layout must be 16-byte aligned");
+  const size_t need = document_layout_ints(batch, seqlen) * sizeof(int32_t);
+  if (layout_bytes < need) return fail(FA2_ERR_INVALID_ARG, "layout must hold %zu bytes", need);
+  const cudaError_t e =
+      launch_document_layout(document_ids, stride_b, batch, seqlen, layout, static_cast<cudaStream_t>(cuda_stream));
+  if (e != cudaSuccess) return fail(FA2_ERR_CUDA, "document layout launch failed: %s", cudaGetErrorString(e));
+  return FA2_OK;
+}
+
+}  // extern "C"
+
+namespace fa2 {
+namespace {
+
+// fa2_fwd, or with `mod` fa2_scored_fwd.
+int fwd_impl(const fa2_fwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
   if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
   const fa2_problem& p = a->p;
   int rc = check_problem(p);
@@ -365,6 +552,13 @@ int fa2_fwd(const fa2_fwd_params* a, void* cuda_stream) {
     return fail(FA2_ERR_INVALID_ARG, "q, k, v, o and lse must be non-null");
   if (a->lse_stride_h < p.seqlen_q || a->lse_stride_b < 0)
     return fail(FA2_ERR_INVALID_ARG, "lse_stride_h must be at least seqlen_q");
+  ScoreModDev mod_dev;
+  int mod_mode = 0;
+  if (mod) {
+    if (a->bias.ptr || a->mask.ptr || a->seqlens || a->dropout_bits)
+      return fail(FA2_ERR_UNSUPPORTED, "bias, mask, seqlens and dropout are not supported in attention with changed scores");
+    if ((rc = make_score_mod(&mod_dev, &mod_mode, *mod, p))) return rc;
+  }
   // First CUDA call of the entry point, on purpose a runtime call: it makes the device's primary
   // context current on a host thread that has not touched the runtime yet (a framework's worker
   // thread served from a memory cache), which the driver-level tensor-map encoder below needs.
@@ -383,7 +577,7 @@ int fa2_fwd(const fa2_fwd_params* a, void* cuda_stream) {
   // group instead of once per query head, by one CTA instead of G. A single row sees every key
   // whether the call is causal or not (bottom-right alignment).
   const int group = p.heads_q / p.heads_kv;
-  const bool pack_heads = can_pack_heads(p) && !a->bias.ptr && !a->mask.ptr && !a->seqlens &&
+  const bool pack_heads = can_pack_heads(p) && !mod && !a->bias.ptr && !a->mask.ptr && !a->seqlens &&
                           a->q_strides.h > 0 && a->o_strides.h > 0;
   int sq_k = p.seqlen_q, hq_k = p.heads_q;
   fa2_strides q_st = a->q_strides, o_st = a->o_strides;
@@ -462,7 +656,9 @@ int fa2_fwd(const fa2_fwd_params* a, void* cuda_stream) {
     try_stage_term(&L.tmMask, &kp.mask, p, 32);
   }
 
-  cudaError_t e = launch_fwd(L, static_cast<cudaStream_t>(cuda_stream));
+  if (mod) kp.mod = mod_dev;
+  cudaError_t e = mod ? launch_fwd_scored(L, mod_mode, static_cast<cudaStream_t>(cuda_stream))
+                      : launch_fwd(L, static_cast<cudaStream_t>(cuda_stream));
   if (e != cudaSuccess)
     return fail(FA2_ERR_CUDA, "forward launch failed: %s", cudaGetErrorString(e));
   if (split) {
@@ -485,28 +681,8 @@ int fa2_fwd(const fa2_fwd_params* a, void* cuda_stream) {
   return FA2_OK;
 }
 
-size_t fa2_fwd_workspace_bytes(const fa2_problem* problem) {
-  if (!problem || check_problem(*problem)) return 0;
-  HeadDim hd;
-  split_head_dim(problem->head_dim, &hd);
-  // whether grouped heads get packed also depends on operands this function does not see
-  // (bias, mask, lengths): report what the larger of the two plans needs
-  size_t need = plan_splits(*problem, hd, false).total;
-  if (can_pack_heads(*problem)) need = std::max(need, plan_splits(*problem, hd, true).total);
-  return need;
-}
-
-size_t fa2_dropout_bits_bytes(const fa2_problem* problem) {
-  if (!problem || check_problem(*problem)) return 0;
-  return dropout_bits_bytes(*problem);
-}
-
-size_t fa2_bwd_workspace_bytes(const fa2_problem* problem) {
-  if (!problem || check_problem(*problem)) return 0;
-  return bwd_workspace(*problem).total;
-}
-
-int fa2_bwd(const fa2_bwd_params* a, void* cuda_stream) {
+// fa2_bwd, or with `mod` fa2_scored_bwd.
+int bwd_impl(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
   if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
   const fa2_problem& p = a->p;
   int rc = check_problem(p);
@@ -530,6 +706,13 @@ int fa2_bwd(const fa2_bwd_params* a, void* cuda_stream) {
       return fail(FA2_ERR_INVALID_ARG, "dbias must be 4-byte aligned");
   }
 
+  ScoreModDev mod_dev;
+  int mod_mode = 0;
+  if (mod) {
+    if (a->bias.ptr || a->mask.ptr || a->seqlens || a->dropout_bits || a->dbias.ptr)
+      return fail(FA2_ERR_UNSUPPORTED, "bias, mask, seqlens and dropout are not supported in attention with changed scores");
+    if ((rc = make_score_mod(&mod_dev, &mod_mode, *mod, p))) return rc;
+  }
   // a runtime call before the driver-level tensor-map encoder: see fa2_fwd
   int* const status_word = status_ptr();
   if (!status_word) return fail(FA2_ERR_CUDA, "status word is not addressable");
@@ -598,7 +781,8 @@ int fa2_bwd(const fa2_bwd_params* a, void* cuda_stream) {
   L.causal = p.causal != 0;
   // (the plain head-dim-128 kernel divides the log-sum-exp by the scale once, in the pre-pass)
   L.feat = kp.bias.ptr || kp.mask.ptr || kp.drop.enabled || !(std::fabs(p.softmax_scale) >= 1e-30f);
-  kp.xstats = (!L.feat && D == 128) ? reinterpret_cast<const uint4*>(ws + w.xstats_off) : nullptr;
+  // (a capped score takes no statistics through the MMAs, see bwd_kernel.cuh)
+  kp.xstats = (!L.feat && D == 128 && !(mod && has_cap(mod_mode))) ? reinterpret_cast<const uint4*>(ws + w.xstats_off) : nullptr;
   kp.dq_order = a->deterministic ? reinterpret_cast<int*>(ws + w.order_off) : nullptr;
   if (L.feat && D == 64) {
     // the head-dim-64 kernel brings 16-bit bias / mask tiles in through the TMA unit
@@ -629,63 +813,13 @@ int fa2_bwd(const fa2_bwd_params* a, void* cuda_stream) {
     L.stage_events[i] = g_bwd_events[i];
     g_bwd_events[i] = nullptr;   // armed for one call only
   }
-  const cudaError_t e = launch_bwd(L, static_cast<cudaStream_t>(cuda_stream));
+  if (mod) kp.mod = mod_dev;
+  const cudaError_t e = mod ? launch_bwd_scored(L, mod_mode, static_cast<cudaStream_t>(cuda_stream))
+                            : launch_bwd(L, static_cast<cudaStream_t>(cuda_stream));
   if (e != cudaSuccess)
     return fail(FA2_ERR_CUDA, "backward launch failed: %s", cudaGetErrorString(e));
   return FA2_OK;
 }
 
-// ---------------------------------------------------------------------------------------------
-// Backward without a caller-provided workspace
-// ---------------------------------------------------------------------------------------------
-namespace {
-// Scratch of the backward (row statistics + fp32 dq accumulator) for callers that cannot hand
-// in device memory of their own. One array per GPU that loads the library, held until exit.
-static __device__ __align__(256) unsigned char g_bwd_static_scratch[FA2_BWD_STATIC_SCRATCH_BYTES];
-
-constexpr int kMaxDevices = 64;
-void* g_static_scratch_ptr[kMaxDevices] = {};
-std::mutex g_static_scratch_mutex;
-
-// Device address of the array on the current device. In host code the array's name is only a
-// handle for the runtime, not an address a kernel could use, so the address is looked up once per
-// device (with that device current) and cached.
-int static_scratch_address(void** out) {
-  int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
-    return fail(FA2_ERR_CUDA, "cannot identify the current CUDA device");
-  std::lock_guard<std::mutex> lock(g_static_scratch_mutex);
-  if (!g_static_scratch_ptr[dev]) {
-    void* ptr = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&ptr, g_bwd_static_scratch);
-    if (e != cudaSuccess || !ptr)
-      return fail(FA2_ERR_CUDA, "cudaGetSymbolAddress failed for the static scratch: %s",
-                  cudaGetErrorString(e));
-    g_static_scratch_ptr[dev] = ptr;
-  }
-  *out = g_static_scratch_ptr[dev];
-  return FA2_OK;
-}
 }  // namespace
-
-int fa2_bwd_static_scratch(const fa2_bwd_params* a, void* cuda_stream) {
-  if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
-  const int rc = check_problem(a->p);
-  if (rc) return rc;
-  const size_t need = bwd_workspace(a->p).total;
-  if (need > static_cast<size_t>(FA2_BWD_STATIC_SCRATCH_BYTES))
-    return fail(FA2_ERR_WORKSPACE,
-                "this problem needs %zu bytes of scratch; the built-in scratch holds %zu bytes "
-                "(batch * heads_q * ceil(seqlen_q/128)*128 * (head_dim + 2) * 4 must not exceed it); "
-                "use fa2_bwd with a workspace instead",
-                need, static_cast<size_t>(FA2_BWD_STATIC_SCRATCH_BYTES));
-  void* scratch = nullptr;
-  const int rs = static_scratch_address(&scratch);
-  if (rs) return rs;
-  fa2_bwd_params b = *a;
-  b.workspace = scratch;
-  b.workspace_bytes = FA2_BWD_STATIC_SCRATCH_BYTES;
-  return fa2_bwd(&b, cuda_stream);
-}
-
-}  // extern "C"
+}  // namespace fa2

@@ -33,4 +33,9 @@ cudaError_t launch_bwd(const BwdLaunch& a, cudaStream_t stream);
 // Head dim 256 variant (64-query steps, one half of the head dim per CTA); called by launch_bwd.
 cudaError_t launch_bwd256(const BwdLaunch& a, cudaStream_t stream);
 
+// Scored variants (score_mod.cuh); mod: kModCap | kModSlope.
+cudaError_t launch_bwd_scored64(const BwdLaunch& a, int mod, cudaStream_t stream);
+cudaError_t launch_bwd_scored128(const BwdLaunch& a, int mod, cudaStream_t stream);
+cudaError_t launch_bwd_scored256(const BwdLaunch& a, int mod, cudaStream_t stream);
+
 }  // namespace fa2

@@ -46,4 +46,9 @@ cudaError_t launch_fwd(const FwdLaunch& a, cudaStream_t stream);
 // Head dim 256 variant (one query tile per CTA, two S buffers); called by launch_fwd.
 cudaError_t launch_fwd256(const FwdLaunch& a, cudaStream_t stream);
 
+// Scored variants (score_mod.cuh); mod: kModCap | kModSlope.
+cudaError_t launch_fwd_scored64(const FwdLaunch& a, int mod, cudaStream_t stream);
+cudaError_t launch_fwd_scored128(const FwdLaunch& a, int mod, cudaStream_t stream);
+cudaError_t launch_fwd_scored256(const FwdLaunch& a, int mod, cudaStream_t stream);
+
 }  // namespace fa2

@@ -172,12 +172,14 @@ struct KeepBitsDropout {
 // `terms(x, kv0)` adds coef * (bias + mask) to the scores (see FeatScale) and `dropout(pk, half)`
 // zeroes the dropped weights of one packed piece (both only with kFeat; see DirectTerms /
 // KeepBitsDropout).
-template <int D, bool kBf16, bool kFeat, class BeforeRescale, class AfterHalf, class Terms, class Dropout>
+// kScored: `terms` changes the scores instead (ModTerms) and the row also has a first visible key, row_first.
+template <int D, bool kBf16, bool kFeat, bool kScored = false, class BeforeRescale, class AfterHalf, class Terms,
+          class Dropout>
 __device__ __forceinline__ void softmax_tile_row(uint32_t tS, uint32_t tO, int j, bool have_o,
                                                  const FwdKernelParams& p, int row_lim, float sc,
                                                  bool prescale, float& m, float& l,
                                                  BeforeRescale before_o_rescale, AfterHalf after_half,
-                                                 Terms terms, Dropout dropout) {
+                                                 Terms terms, Dropout dropout, int row_first = 0) {
   tc_fence_after();
   float x[kBN];
   {
@@ -195,10 +197,16 @@ __device__ __forceinline__ void softmax_tile_row(uint32_t tS, uint32_t tO, int j
     }
     terms(x, kv0);
   }
+  if constexpr (kScored) terms(x, kv0);
   if (kv0 + kBN - 1 > row_lim) {   // boundary tile for this row: causal edge or key padding
 #pragma unroll
     for (int c = 0; c < kBN; ++c)
       if (kv0 + c > row_lim) x[c] = -INFINITY;
+  }
+  if (kScored && kv0 < row_first) {   // the row's document begins inside this tile or behind it
+#pragma unroll
+    for (int c = 0; c < kBN; ++c)
+      if (kv0 + c < row_first) x[c] = -INFINITY;
   }
   float mx0 = fmaxf(x[0], x[1]), mx1 = fmaxf(x[2], x[3]), mx2 = fmaxf(x[4], x[5]),
         mx3 = fmaxf(x[6], x[7]);

@@ -67,6 +67,19 @@ __device__ __forceinline__ uint32_t dropout_bh_index(const DropoutDev& d, int b,
   return static_cast<uint32_t>((b_off + b) * d.hq_global + h_off + h);
 }
 
+// Changes of the scores and of what a query sees (the scored kernels, score_mod.cuh).
+struct ScoreModDev {
+  float cap2;             // cap * log2(e)
+  float arg2;             // 2 * softmax_scale * log2(e) / cap
+  const float* slopes;    // [Hq] distance slopes, or null
+  const int* prefix_lens; // [B], or null
+  int causal;
+  // Document layout, or null: for every token the first and one past the last token of its document
+  // (0, 0 for padding), and the same over every 128 tokens (least first, greatest end)
+  const int *tok_lo, *tok_hi;     // [B][Sq]
+  const int *tile_lo, *tile_hi;   // [B][ceil(Sq / 128)]
+};
+
 struct FwdKernelParams {
   int B, Sq, Sk, Hq, Hkv, G;
   int causal_off;       // Sk - Sq: query row i may see key j iff j <= i + causal_off
@@ -90,6 +103,7 @@ struct FwdKernelParams {
   // [n_splits * B][Sq][Hq][kernel head dim]; the 16-bit output is then written by the merge alone.
   float* part_o;
   int* status;          // device status word (bounded-wait time-outs)
+  ScoreModDev mod;      // read by the scored kernels alone
 };
 
 struct BwdKernelParams;
@@ -145,6 +159,7 @@ struct BwdKernelParams {
   // descending too, so that a block only waits for blocks with a lower index.
   int* dq_order;
   int* status;
+  ScoreModDev mod;      // read by the scored kernels alone
 };
 
 }  // namespace fa2

@@ -13,6 +13,12 @@ from ._kernel_calls import (
     dropout_bits_buffer,
     fwd_attention_kernel_call,
 )
+from ._scored_attention import (
+    bwd_scored_attention_kernel_call,
+    document_layout,
+    fwd_scored_attention_kernel_call,
+    scored_flash_attention,
+)
 
 __all__ = (
     "AttentionConfig",
@@ -25,5 +31,9 @@ __all__ = (
     "bwd_attention_kernel_call",
     "device_status",
     "dropout_bits_buffer",
+    "scored_flash_attention",
+    "document_layout",
+    "fwd_scored_attention_kernel_call",
+    "bwd_scored_attention_kernel_call",
 )
 __version__ = "0.1.0"

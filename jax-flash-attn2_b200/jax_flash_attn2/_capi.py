@@ -29,9 +29,19 @@ EXPORTED_SYMBOLS = (
     "fa2_bwd_static_scratch",
     "fa2_dropout_bits_bytes",
 )
+# operators of fa2_b200_lm.h (score changes, paged cache)
+LM_EXPORTED_SYMBOLS = (
+    "fa2_lm_version",
+    "fa2_document_layout_bytes",
+    "fa2_document_layout",
+    "fa2_scored_fwd",
+    "fa2_scored_bwd",
+)
 FA2_BWD_STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 # FA2_ABI_VERSION of the header these structures were written against (major * 1000 + minor)
 FA2_ABI_VERSION = 3000
+# the same for fa2_b200_lm.h
+FA2_LM_ABI_VERSION = 1000
 
 
 class Strides(C.Structure):
@@ -120,6 +130,15 @@ class BwdParams(C.Structure):
     ]
 
 
+class ScoreMod(C.Structure):
+    _fields_ = [
+        ("softcap", C.c_float),
+        ("alibi_slopes", C.c_void_p),
+        ("prefix_lens", C.c_void_p),
+        ("document_layout", C.c_void_p),
+    ]
+
+
 class Fa2Error(RuntimeError):
     """A call into libfa2_b200.so returned a non-zero status."""
 
@@ -151,6 +170,12 @@ def load() -> C.CDLL:
             f"{LIB_PATH} reports ABI version {found}, this binding needs {FA2_ABI_VERSION}: rebuild it with "
             f"`python {os.path.join(_PKG_ROOT, 'build.py')} --force`."
         )
+    if not hasattr(lib, "fa2_lm_version") or lib.fa2_lm_version() // 1000 != FA2_LM_ABI_VERSION // 1000 \
+            or lib.fa2_lm_version() < FA2_LM_ABI_VERSION:
+        raise ImportError(
+            f"{LIB_PATH} lacks version {FA2_LM_ABI_VERSION} of the language model operators: rebuild it with "
+            f"`python {os.path.join(_PKG_ROOT, 'build.py')} --force`."
+        )
     lib.fa2_fwd.argtypes = [C.POINTER(FwdParams), C.c_void_p]
     lib.fa2_fwd.restype = C.c_int
     lib.fa2_bwd.argtypes = [C.POINTER(BwdParams), C.c_void_p]
@@ -169,6 +194,14 @@ def load() -> C.CDLL:
     lib.fa2_bwd_static_scratch.restype = C.c_int
     lib.fa2_debug_bwd_stage_events.argtypes = [C.POINTER(C.c_void_p)]
     lib.fa2_debug_bwd_stage_events.restype = C.c_int
+    lib.fa2_document_layout_bytes.argtypes = [C.c_int32, C.c_int32]
+    lib.fa2_document_layout_bytes.restype = C.c_size_t
+    lib.fa2_document_layout.argtypes = [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.fa2_document_layout.restype = C.c_int
+    lib.fa2_scored_fwd.argtypes = [C.POINTER(FwdParams), C.POINTER(ScoreMod), C.c_void_p]
+    lib.fa2_scored_fwd.restype = C.c_int
+    lib.fa2_scored_bwd.argtypes = [C.POINTER(BwdParams), C.POINTER(ScoreMod), C.c_void_p]
+    lib.fa2_scored_bwd.restype = C.c_int
     _lib = lib
     return lib
 

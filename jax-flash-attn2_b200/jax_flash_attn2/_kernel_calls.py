@@ -24,23 +24,24 @@ _DTYPE_CODE = {torch.float16: _capi.FA2_FP16, torch.bfloat16: _capi.FA2_BF16, to
 _raw_stream_fn = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _launch(fn, params, device: torch.device) -> None:
+def _launch(fn, params, device: torch.device, *more) -> None:
     """Calls one C-ABI entry point on torch's current stream of `device`. The device is only
     switched when it is not the current one, and the stream handle is taken through the raw
-    accessor when torch has it: for small problems the host side of a call is what one waits for."""
+    accessor when torch has it: for small problems the host side of a call is what one waits for.
+    `more`: further parameter blocks, passed by reference behind the first."""
     index = device.index
     current = torch.cuda.current_device()
     if index is None:
         index = current
     if index != current:
         with torch.cuda.device(index):
-            _launch(fn, params, device)
+            _launch(fn, params, device, *more)
         return
     if _raw_stream_fn is not None:
         stream = _raw_stream_fn(index)
     else:
         stream = torch.cuda.current_stream(index).cuda_stream
-    _capi.check(fn(C.byref(params), C.c_void_p(stream)))
+    _capi.check(fn(C.byref(params), *(C.byref(x) for x in more), C.c_void_p(stream)))
 
 
 def _strides(x: torch.Tensor) -> _capi.Strides:
