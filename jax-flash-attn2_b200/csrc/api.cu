@@ -537,6 +537,264 @@ int fa2_document_layout(const int32_t* document_ids, int64_t stride_b, int32_t b
   return FA2_OK;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Serving with a paged cache (fa2_b200_lm.h)
+// ---------------------------------------------------------------------------------------------
+namespace {
+constexpr int kMaxRequests = 8192;
+constexpr int64_t kMaxContext = 1 << 30;   // keys a table can hold: positions and tile counts stay within 32 bits
+
+int check_groups(int32_t heads_q, int32_t heads_kv) {
+  if (heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0)
+    return fail(FA2_ERR_INVALID_ARG, "query heads (%d) must be divisible by key/value heads (%d)", heads_q, heads_kv);
+  if (heads_q / heads_kv > 128)
+    return fail(FA2_ERR_UNSUPPORTED, "at most 128 query heads per key/value head are supported");
+  return FA2_OK;
+}
+// log2 of a page size, or -1
+int page_shift_of(int32_t page_size) {
+  if (page_size < 8 || page_size > (1 << 20) || (page_size & (page_size - 1))) return -1;
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+int item_tokens_of(int32_t heads_q, int32_t heads_kv) { return 2 * (128 / (heads_q / heads_kv)); }
+int64_t max_items(int64_t requests, int64_t tokens, int64_t item_tokens) {
+  return std::min(tokens, tokens / item_tokens + requests);
+}
+
+int check_cache(const fa2_paged_cache& c, const char* what) {
+  if (!c.ptr) return fail(FA2_ERR_INVALID_ARG, "%s must be non-null", what);
+  if (reinterpret_cast<uintptr_t>(c.ptr) & 15) return fail(FA2_ERR_UNSUPPORTED, "%s: pointer must be 16-byte aligned", what);
+  if (c.stride_page <= 0 || c.stride_slot <= 0 || c.stride_head <= 0)
+    return fail(FA2_ERR_INVALID_ARG, "%s: strides must be positive", what);
+  if ((c.stride_page % 8) || (c.stride_slot % 8) || (c.stride_head % 8))
+    return fail(FA2_ERR_UNSUPPORTED, "%s: strides must be multiples of 8 elements", what);
+  return FA2_OK;
+}
+
+// 5-D map of 16-bit elements with a 128-byte swizzle.
+int encode_map(CUtensorMap* tm, const void* ptr, bool bf16, const cuuint64_t (&dims)[5], const cuuint64_t (&strides)[4],
+               const cuuint32_t (&box)[5], const char* what) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(FA2_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                         const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FA2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", what, static_cast<int>(r));
+  return FA2_OK;
+}
+}  // namespace
+
+size_t fa2_paged_work_bytes(int32_t requests, int32_t num_tokens, int32_t heads_q, int32_t heads_kv) {
+  if (requests <= 0 || num_tokens < 0 || check_groups(heads_q, heads_kv)) return 0;
+  return (kWorkHeader + kWorkItem * static_cast<size_t>(max_items(requests, num_tokens, item_tokens_of(heads_q, heads_kv)))) *
+         sizeof(int32_t);
+}
+
+int fa2_paged_plan(const fa2_paged_plan_params* a, void* cuda_stream) {
+  if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
+  if (a->requests <= 0 || a->num_tokens < 0 || a->table_width <= 0 || a->n_free < 0)
+    return fail(FA2_ERR_INVALID_ARG, "requests and table_width must be positive, num_tokens and n_free not negative");
+  if (a->requests > kMaxRequests) return fail(FA2_ERR_UNSUPPORTED, "at most %d requests are supported", kMaxRequests);
+  const int rc = check_groups(a->heads_q, a->heads_kv);
+  if (rc) return rc;
+  const int shift = page_shift_of(a->page_size);
+  if (shift < 0) return fail(FA2_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 2^20");
+  if (!a->context_lens || !a->new_lens || !a->block_table || (!a->free_pages && a->n_free > 0) || !a->cu_seqlens ||
+      !a->seqlens_k || (a->num_tokens > 0 && (!a->slot_map || !a->positions)) || !a->pages_taken || !a->work)
+    return fail(FA2_ERR_INVALID_ARG, "the plan's arrays must be non-null");
+  if (a->table_stride < a->table_width) return fail(FA2_ERR_INVALID_ARG, "table_stride must be at least table_width");
+  if ((static_cast<int64_t>(a->table_width) << shift) > kMaxContext)
+    return fail(FA2_ERR_UNSUPPORTED, "table_width * page_size must not exceed 2^30");
+  if ((reinterpret_cast<uintptr_t>(a->context_lens) | reinterpret_cast<uintptr_t>(a->new_lens) |
+       reinterpret_cast<uintptr_t>(a->block_table) | reinterpret_cast<uintptr_t>(a->free_pages) |
+       reinterpret_cast<uintptr_t>(a->free_start) | reinterpret_cast<uintptr_t>(a->cu_seqlens) |
+       reinterpret_cast<uintptr_t>(a->seqlens_k) | reinterpret_cast<uintptr_t>(a->positions) |
+       reinterpret_cast<uintptr_t>(a->pages_taken)) & 3)
+    return fail(FA2_ERR_INVALID_ARG, "the plan's int32 arrays must be 4-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a->slot_map) & 7) || (reinterpret_cast<uintptr_t>(a->work) & 15))
+    return fail(FA2_ERR_INVALID_ARG, "slot_map must be 8-byte and work 16-byte aligned");
+  const int item_tokens = item_tokens_of(a->heads_q, a->heads_kv);
+  const int64_t items = max_items(a->requests, a->num_tokens, item_tokens);
+  if (a->work_bytes < (kWorkHeader + kWorkItem * static_cast<size_t>(items)) * sizeof(int32_t))
+    return fail(FA2_ERR_WORKSPACE, "work must hold fa2_paged_work_bytes bytes");
+  const int64_t tiles = ((static_cast<int64_t>(a->table_width) << shift) + 127) / 128;
+  if (items * tiles > INT_MAX)
+    return fail(FA2_ERR_UNSUPPORTED, "problem too large: %lld items of up to %lld key tiles must stay below 2^31",
+                static_cast<long long>(items), static_cast<long long>(tiles));
+  PagedPlanDev d;
+  d.context_lens = a->context_lens;
+  d.new_lens = a->new_lens;
+  d.B = a->requests;
+  d.block_table = a->block_table;
+  d.table_stride = a->table_stride;
+  d.table_width = a->table_width;
+  d.free_pages = a->free_pages;
+  d.n_free = a->n_free;
+  d.free_start = a->free_start;
+  d.page_shift = shift;
+  d.num_tokens = a->num_tokens;
+  d.item_tokens = item_tokens;
+  d.cu_seqlens = a->cu_seqlens;
+  d.seqlens_k = a->seqlens_k;
+  d.slot_map = reinterpret_cast<long long*>(a->slot_map);
+  d.positions = a->positions;
+  d.pages_taken = a->pages_taken;
+  d.work = a->work;
+  const cudaError_t e = launch_paged_plan(d, static_cast<cudaStream_t>(cuda_stream));
+  if (e != cudaSuccess) return fail(FA2_ERR_CUDA, "plan launch failed: %s", cudaGetErrorString(e));
+  return FA2_OK;
+}
+
+int fa2_paged_cache_write(const fa2_paged_write_params* a, void* cuda_stream) {
+  if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
+  if (a->tokens < 0 || a->heads <= 0 || a->head_dim <= 0 || a->pages <= 0)
+    return fail(FA2_ERR_INVALID_ARG, "heads, head_dim and pages must be positive, tokens not negative");
+  const int shift = page_shift_of(a->page_size);
+  if (shift < 0) return fail(FA2_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 2^20");
+  if (a->head_dim % 8) return fail(FA2_ERR_UNSUPPORTED, "head_dim must be a multiple of 8");
+  int rc = check_cache(a->k_cache, "k_cache");
+  if (!rc) rc = check_cache(a->v_cache, "v_cache");
+  if (rc) return rc;
+  if (a->tokens == 0) return FA2_OK;
+  if (!a->k || !a->v || !a->slot_map) return fail(FA2_ERR_INVALID_ARG, "k, v and slot_map must be non-null");
+  if ((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15)
+    return fail(FA2_ERR_UNSUPPORTED, "k and v must be 16-byte aligned");
+  if ((a->k_stride_t % 8) || (a->k_stride_h % 8) || (a->v_stride_t % 8) || (a->v_stride_h % 8))
+    return fail(FA2_ERR_UNSUPPORTED, "k and v: strides must be multiples of 8 elements");
+  if (a->k_stride_t < 0 || a->k_stride_h < 0 || a->v_stride_t < 0 || a->v_stride_h < 0)
+    return fail(FA2_ERR_INVALID_ARG, "k and v: strides must not be negative");
+  if (reinterpret_cast<uintptr_t>(a->slot_map) & 7) return fail(FA2_ERR_INVALID_ARG, "slot_map must be 8-byte aligned");
+  const int64_t per_token = static_cast<int64_t>(a->heads) * (a->head_dim / 8);
+  if (per_token > INT_MAX || a->tokens * per_token > 256LL * INT_MAX)
+    return fail(FA2_ERR_UNSUPPORTED, "tokens * heads * head_dim is too large");
+  PagedWriteDev d;
+  d.k = static_cast<const uint16_t*>(a->k);
+  d.v = static_cast<const uint16_t*>(a->v);
+  d.k_st = a->k_stride_t; d.k_sh = a->k_stride_h;
+  d.v_st = a->v_stride_t; d.v_sh = a->v_stride_h;
+  d.k_cache = static_cast<uint16_t*>(const_cast<void*>(a->k_cache.ptr));
+  d.v_cache = static_cast<uint16_t*>(const_cast<void*>(a->v_cache.ptr));
+  d.kc_sp = a->k_cache.stride_page; d.kc_ss = a->k_cache.stride_slot; d.kc_sh = a->k_cache.stride_head;
+  d.vc_sp = a->v_cache.stride_page; d.vc_ss = a->v_cache.stride_slot; d.vc_sh = a->v_cache.stride_head;
+  d.slot_map = reinterpret_cast<const long long*>(a->slot_map);
+  d.slots = static_cast<long long>(a->pages) << shift;
+  d.tokens = a->tokens;
+  d.heads = a->heads;
+  d.chunks_per_head = a->head_dim / 8;
+  d.page_shift = shift;
+  const cudaError_t e = launch_paged_write(d, static_cast<cudaStream_t>(cuda_stream));
+  if (e != cudaSuccess) return fail(FA2_ERR_CUDA, "cache write launch failed: %s", cudaGetErrorString(e));
+  return FA2_OK;
+}
+
+size_t fa2_paged_workspace_bytes(int32_t head_dim) {
+  HeadDim hd;
+  if (!split_head_dim(head_dim, &hd) || hd.padded > 128) return 0;
+  // two partial items of 256 rows per CTA: the rows, then their log-sum-exp
+  return static_cast<size_t>(2) * sm_count() * 256 * (hd.padded + 1) * sizeof(float);
+}
+
+int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) {
+  if (!a) return fail(FA2_ERR_INVALID_ARG, "params is null");
+  if (a->tokens < 0 || a->requests <= 0 || a->table_width <= 0 || a->pages <= 0)
+    return fail(FA2_ERR_INVALID_ARG, "requests, table_width and pages must be positive, tokens not negative");
+  int rc = check_groups(a->heads_q, a->heads_kv);
+  if (rc) return rc;
+  if (a->dtype != FA2_FP16 && a->dtype != FA2_BF16)
+    return fail(FA2_ERR_UNSUPPORTED, "only fp16 and bf16 inputs are supported");
+  HeadDim hd;
+  if (!split_head_dim(a->head_dim, &hd) || hd.padded > 128)
+    return fail(FA2_ERR_UNSUPPORTED, "head_dim %d is not supported (multiples of 8 up to 64, of 16 up to 128 are)", a->head_dim);
+  const int shift = page_shift_of(a->page_size);
+  if (shift < 0) return fail(FA2_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 2^20");
+  if ((static_cast<int64_t>(a->table_width) << shift) > kMaxContext)
+    return fail(FA2_ERR_UNSUPPORTED, "table_width * page_size must not exceed 2^30");
+  if (!(a->softmax_scale >= 1e-30f) || !std::isfinite(a->softmax_scale))
+    return fail(FA2_ERR_INVALID_ARG, "softmax_scale must be positive and finite");
+  if ((rc = check_softcap(a->softcap))) return rc;
+  if ((rc = check_cache(a->k_cache, "k_cache")) || (rc = check_cache(a->v_cache, "v_cache"))) return rc;
+  if (a->tokens == 0) return FA2_OK;
+  if (!a->q || !a->o || !a->block_table || !a->work)
+    return fail(FA2_ERR_INVALID_ARG, "q, o, block_table and work must be non-null");
+  if (a->table_stride < a->table_width) return fail(FA2_ERR_INVALID_ARG, "table_stride must be at least table_width");
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->o)) & 15)
+    return fail(FA2_ERR_UNSUPPORTED, "q and o must be 16-byte aligned");
+  if ((a->q_stride_t % 8) || (a->q_stride_h % 8) || (a->o_stride_t % 8) || (a->o_stride_h % 8))
+    return fail(FA2_ERR_UNSUPPORTED, "q and o: strides must be multiples of 8 elements");
+  if (a->q_stride_t <= 0 || a->q_stride_h <= 0 || a->o_stride_t <= 0 || a->o_stride_h <= 0)
+    return fail(FA2_ERR_INVALID_ARG, "q and o: strides must be positive");
+  if ((reinterpret_cast<uintptr_t>(a->work) & 15) || ((reinterpret_cast<uintptr_t>(a->block_table) |
+       reinterpret_cast<uintptr_t>(a->lse) | reinterpret_cast<uintptr_t>(a->alibi_slopes)) & 3))
+    return fail(FA2_ERR_INVALID_ARG, "work must be 16-byte, block_table, lse and alibi_slopes 4-byte aligned");
+  // a runtime call before the driver-level tensor-map encoder: see fwd_impl
+  int* const status_word = status_ptr();
+  if (!status_word) return fail(FA2_ERR_CUDA, "status word is not addressable");
+  const size_t need = fa2_paged_workspace_bytes(a->head_dim);
+  if (!a->workspace || a->workspace_bytes < need) return fail(FA2_ERR_WORKSPACE, "workspace must hold %zu bytes", need);
+  if (reinterpret_cast<uintptr_t>(a->workspace) & (kWorkspaceAlign - 1))
+    return fail(FA2_ERR_WORKSPACE, "workspace must be 128-byte aligned");
+
+  PagedAttnLaunch L;
+  std::memset(&L, 0, sizeof(L));
+  const bool bf16 = a->dtype == FA2_BF16;
+  const int group = a->heads_q / a->heads_kv, tile_tokens = 128 / group;
+  const auto bytes = [](int64_t elements) { return static_cast<cuuint64_t>(elements) * 2; };
+  {
+    // (columns, heads of a group, tokens, column blocks, key/value heads): a box is the rows of one query tile
+    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(hd.blk), static_cast<cuuint64_t>(group),
+                                static_cast<cuuint64_t>(a->tokens), static_cast<cuuint64_t>(hd.nblk),
+                                static_cast<cuuint64_t>(a->heads_kv)};
+    const cuuint64_t st[4] = {bytes(a->q_stride_h), bytes(a->q_stride_t), bytes(hd.blk), bytes(a->q_stride_h * group)};
+    const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tile_tokens), 1, 1};
+    if ((rc = encode_map(&L.tmQ, a->q, bf16, dims, st, box, "q"))) return rc;
+  }
+  for (int x = 0; x < 2; ++x) {
+    // (columns, places in a page, column blocks, heads, pages): a box is a piece of a page of at most 128 rows
+    const fa2_paged_cache& c = x ? a->v_cache : a->k_cache;
+    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(hd.blk), static_cast<cuuint64_t>(a->page_size),
+                                static_cast<cuuint64_t>(hd.nblk), static_cast<cuuint64_t>(a->heads_kv),
+                                static_cast<cuuint64_t>(a->pages)};
+    const cuuint64_t st[4] = {bytes(c.stride_slot), bytes(hd.blk), bytes(c.stride_head), bytes(c.stride_page)};
+    const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(std::min(a->page_size, 128)), 1, 1, 1};
+    if ((rc = encode_map(x ? &L.tmV : &L.tmK, c.ptr, bf16, dims, st, box, x ? "v_cache" : "k_cache"))) return rc;
+  }
+  PagedAttnDev& d = L.p;
+  d.T = a->tokens; d.Hq = a->heads_q; d.Hkv = a->heads_kv; d.G = group;
+  d.tile_tokens = tile_tokens;
+  d.work = a->work;
+  d.block_table = a->block_table;
+  d.table_stride = a->table_stride;
+  d.table_width = a->table_width;
+  d.page_shift = shift;
+  d.num_pages = a->pages;
+  d.scale_log2 = static_cast<float>(a->softmax_scale * 1.4426950408889634);
+  L.mod = 0;
+  if (a->softcap > 0.f) {
+    L.mod |= kModCap;
+    d.cap2 = static_cast<float>(a->softcap * 1.4426950408889634);
+    d.arg2 = static_cast<float>(2.0 * a->softmax_scale * 1.4426950408889634 / a->softcap);
+    if (!std::isfinite(d.arg2)) return fail(FA2_ERR_INVALID_ARG, "softmax_scale / softcap overflows");
+  }
+  if (a->alibi_slopes) L.mod |= kModSlope;
+  d.slopes = a->alibi_slopes;
+  d.out = static_cast<uint16_t*>(a->o);
+  d.out_st = a->o_stride_t; d.out_sh = a->o_stride_h;
+  d.blk = hd.blk;
+  d.lse = a->lse;
+  d.part_o = static_cast<float*>(a->workspace);
+  d.part_lse = d.part_o + static_cast<size_t>(2) * sm_count() * 256 * hd.padded;
+  d.status = status_word;
+  L.head_dim = hd.padded;
+  L.bf16 = bf16;
+  const cudaError_t e = launch_paged_attention(L, static_cast<cudaStream_t>(cuda_stream));
+  if (e != cudaSuccess) return fail(FA2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));
+  return FA2_OK;
+}
+
 }  // extern "C"
 
 namespace fa2 {

@@ -1,10 +1,74 @@
-// Host-side launchers of the operators declared in fa2_b200_lm.h.
+// Host-side launch records of the operators declared in fa2_b200_lm.h.
 #pragma once
+#include <cstdint>
+
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace fa2 {
 
 cudaError_t launch_document_layout(const int* ids, long long stride_b, int B, int S, int* layout, cudaStream_t stream);
+
+// Work list of the paged attention (int32): a header of kWorkHeader words (0: items, 1: key tiles of all items
+// together), then kWorkItem words per item: first row of the packed tensors, tokens, position of the first token,
+// request, key tiles of the items before it, key tiles of its own, 0, 0.
+constexpr int kWorkHeader = 16;
+constexpr int kWorkItem = 8;
+
+struct PagedPlanDev {
+  const int *context_lens, *new_lens;
+  int B;
+  int* block_table;
+  long long table_stride;
+  int table_width;
+  const int* free_pages;
+  int n_free;
+  const int* free_start;     // or null: 0
+  int page_shift;
+  int num_tokens;
+  int item_tokens;           // query tokens per item of the work list
+  int *cu_seqlens, *seqlens_k;
+  long long* slot_map;
+  int *positions, *pages_taken, *work;
+};
+cudaError_t launch_paged_plan(const PagedPlanDev& p, cudaStream_t stream);
+
+struct PagedWriteDev {
+  const uint16_t *k, *v;
+  long long k_st, k_sh, v_st, v_sh;               // (token, head) element strides
+  uint16_t *k_cache, *v_cache;
+  long long kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh;   // (page, slot, head) element strides
+  const long long* slot_map;
+  long long slots;                                 // slots of the cache: pages << page_shift
+  int tokens, heads, chunks_per_head;              // chunks of 8 elements
+  int page_shift;
+};
+cudaError_t launch_paged_write(const PagedWriteDev& p, cudaStream_t stream);
+
+struct PagedAttnDev {
+  int T, Hq, Hkv, G;
+  int tile_tokens;           // tokens of a 128-row tile: floor(128 / G)
+  const int* work;
+  const int* block_table;
+  long long table_stride;
+  int table_width, page_shift, num_pages;
+  float scale_log2, cap2, arg2;
+  const float* slopes;       // [Hq] or null
+  uint16_t* out;
+  long long out_st, out_sh;  // (token, head) element strides
+  int blk;                   // real columns in each 64-column block
+  float* lse;                // [T][Hq] natural log, or null
+  float* part_o;             // [2 * CTAs][256][kernel head dim]
+  float* part_lse;           // [2 * CTAs][256], log2
+  int* status;
+};
+struct PagedAttnLaunch {
+  CUtensorMap tmQ, tmK, tmV;
+  PagedAttnDev p;
+  int head_dim;              // 64 or 128
+  bool bf16;
+  int mod;                   // kModCap | kModSlope
+};
+cudaError_t launch_paged_attention(const PagedAttnLaunch& a, cudaStream_t stream);
 
 }  // namespace fa2

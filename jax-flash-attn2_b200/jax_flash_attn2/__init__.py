@@ -13,6 +13,7 @@ from ._kernel_calls import (
     dropout_bits_buffer,
     fwd_attention_kernel_call,
 )
+from ._paged import PagedStepPlan, paged_attention, paged_cache_write, paged_step_plan
 from ._scored_attention import (
     bwd_scored_attention_kernel_call,
     document_layout,
@@ -32,6 +33,10 @@ __all__ = (
     "device_status",
     "dropout_bits_buffer",
     "scored_flash_attention",
+    "PagedStepPlan",
+    "paged_step_plan",
+    "paged_cache_write",
+    "paged_attention",
     "document_layout",
     "fwd_scored_attention_kernel_call",
     "bwd_scored_attention_kernel_call",

@@ -36,6 +36,11 @@ LM_EXPORTED_SYMBOLS = (
     "fa2_document_layout",
     "fa2_scored_fwd",
     "fa2_scored_bwd",
+    "fa2_paged_work_bytes",
+    "fa2_paged_plan",
+    "fa2_paged_cache_write",
+    "fa2_paged_workspace_bytes",
+    "fa2_paged_attention",
 )
 FA2_BWD_STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 # FA2_ABI_VERSION of the header these structures were written against (major * 1000 + minor)
@@ -139,6 +144,58 @@ class ScoreMod(C.Structure):
     ]
 
 
+class PagedPlanParams(C.Structure):
+    _fields_ = [
+        ("context_lens", C.c_void_p), ("new_lens", C.c_void_p),
+        ("requests", C.c_int32),
+        ("block_table", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("free_pages", C.c_void_p),
+        ("n_free", C.c_int32),
+        ("free_start", C.c_void_p),
+        ("page_size", C.c_int32), ("num_tokens", C.c_int32),
+        ("heads_q", C.c_int32), ("heads_kv", C.c_int32),
+        ("cu_seqlens", C.c_void_p),
+        ("seqlens_k", C.c_void_p),
+        ("slot_map", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("pages_taken", C.c_void_p),
+        ("work", C.c_void_p),
+        ("work_bytes", C.c_size_t),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_page", C.c_int64), ("stride_slot", C.c_int64), ("stride_head", C.c_int64)]
+
+
+class PagedWriteParams(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v", C.c_void_p), ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
+        ("k_cache", PagedCache), ("v_cache", PagedCache),
+        ("slot_map", C.c_void_p),
+        ("tokens", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32),
+    ]
+
+
+class PagedAttentionParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+        ("o", C.c_void_p), ("o_stride_t", C.c_int64), ("o_stride_h", C.c_int64),
+        ("lse", C.c_void_p),
+        ("k_cache", PagedCache), ("v_cache", PagedCache),
+        ("tokens", C.c_int32), ("heads_q", C.c_int32), ("heads_kv", C.c_int32), ("head_dim", C.c_int32),
+        ("dtype", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int32), ("requests", C.c_int32),
+        ("work", C.c_void_p),
+        ("softmax_scale", C.c_float), ("softcap", C.c_float),
+        ("alibi_slopes", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 class Fa2Error(RuntimeError):
     """A call into libfa2_b200.so returned a non-zero status."""
 
@@ -202,6 +259,15 @@ def load() -> C.CDLL:
     lib.fa2_scored_fwd.restype = C.c_int
     lib.fa2_scored_bwd.argtypes = [C.POINTER(BwdParams), C.POINTER(ScoreMod), C.c_void_p]
     lib.fa2_scored_bwd.restype = C.c_int
+    lib.fa2_paged_work_bytes.argtypes = [C.c_int32] * 4
+    lib.fa2_paged_work_bytes.restype = C.c_size_t
+    lib.fa2_paged_workspace_bytes.argtypes = [C.c_int32]
+    lib.fa2_paged_workspace_bytes.restype = C.c_size_t
+    for name, params in (("fa2_paged_plan", PagedPlanParams), ("fa2_paged_cache_write", PagedWriteParams),
+                         ("fa2_paged_attention", PagedAttentionParams)):
+        fn = getattr(lib, name)
+        fn.argtypes = [C.POINTER(params), C.c_void_p]
+        fn.restype = C.c_int
     _lib = lib
     return lib
 

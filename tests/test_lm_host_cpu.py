@@ -139,3 +139,131 @@ def test_scored_oracle_agrees_with_the_dense_one_and_with_automatic_differentiat
     r = scored.attention(q, k, v, seen, softcap=2.0, alibi_slopes=slopes, dO=do)
     for name, x in zip(("dq", "dk", "dv"), auto):
         torch.testing.assert_close(r[name], x)
+
+
+def _plan_params():
+    lib = _capi.load()
+    a = _capi.PagedPlanParams()
+    a.requests, a.table_width, a.table_stride, a.n_free, a.page_size, a.num_tokens, a.heads_q, a.heads_kv = 3, 5, 5, 4, 16, 100, 8, 2
+    for name in ("context_lens", "new_lens", "block_table", "free_pages", "cu_seqlens", "seqlens_k", "slot_map", "positions", "pages_taken", "work"):
+        setattr(a, name, 0x10000)
+    a.work_bytes = lib.fa2_paged_work_bytes(3, 100, 8, 2)
+    return a
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(requests=0), _capi.FA2_ERR_INVALID_ARG, b"positive"),
+    (dict(requests=8193), _capi.FA2_ERR_UNSUPPORTED, b"8192"),
+    (dict(num_tokens=-1), _capi.FA2_ERR_INVALID_ARG, b"negative"),
+    (dict(page_size=24), _capi.FA2_ERR_UNSUPPORTED, b"power of two"),
+    (dict(page_size=4), _capi.FA2_ERR_UNSUPPORTED, b"power of two"),
+    (dict(page_size=2 ** 21), _capi.FA2_ERR_UNSUPPORTED, b"power of two"),
+    (dict(heads_q=3), _capi.FA2_ERR_INVALID_ARG, b"divisible"),
+    (dict(heads_q=129, heads_kv=1), _capi.FA2_ERR_UNSUPPORTED, b"128"),
+    (dict(table_stride=4), _capi.FA2_ERR_INVALID_ARG, b"table_stride"),
+    (dict(table_width=2 ** 27, table_stride=2 ** 27), _capi.FA2_ERR_UNSUPPORTED, b"2^30"),
+    (dict(slot_map=None), _capi.FA2_ERR_INVALID_ARG, b"non-null"),
+    (dict(free_pages=None), _capi.FA2_ERR_INVALID_ARG, b"non-null"),
+    (dict(work=0x10008), _capi.FA2_ERR_INVALID_ARG, b"16-byte"),
+    (dict(slot_map=0x10004), _capi.FA2_ERR_INVALID_ARG, b"8-byte"),
+    (dict(context_lens=0x10002), _capi.FA2_ERR_INVALID_ARG, b"4-byte"),
+    (dict(work_bytes=16), _capi.FA2_ERR_WORKSPACE, b"work"),
+    (dict(num_tokens=2 ** 30, heads_q=128, heads_kv=1, table_width=2 ** 20, table_stride=2 ** 20, work_bytes=2 ** 40), _capi.FA2_ERR_UNSUPPORTED, b"too large"),
+])
+def test_plan_refusals(change, code, word):
+    a = _plan_params()
+    for name, x in change.items():
+        setattr(a, name, x)
+    lib = _capi.load()
+    assert lib.fa2_paged_plan(C.byref(a), None) == code
+    assert word in lib.fa2_last_error()
+
+
+def test_paged_sizes():
+    lib = _capi.load()
+    assert lib.fa2_paged_work_bytes(3, 100, 8, 2) == 4 * (16 + 8 * (100 // 64 + 3))      # 64 tokens of 4 heads per item
+    assert lib.fa2_paged_work_bytes(200, 100, 8, 8) == 4 * (16 + 8 * 100)                # at most one item per token
+    assert lib.fa2_paged_work_bytes(3, 100, 3, 2) == 0
+    assert lib.fa2_paged_workspace_bytes(256) == 0 and lib.fa2_paged_workspace_bytes(20) == 0
+    assert lib.fa2_paged_workspace_bytes(128) % (2 * 256 * 129 * 4) == 0
+
+
+def _set_cache(c):
+    c.ptr, c.stride_page, c.stride_slot, c.stride_head = 0x10000, 16 * 2 * 64, 2 * 64, 64
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(tokens=-1), _capi.FA2_ERR_INVALID_ARG, b"negative"),
+    (dict(head_dim=20), _capi.FA2_ERR_UNSUPPORTED, b"multiple of 8"),
+    (dict(page_size=12), _capi.FA2_ERR_UNSUPPORTED, b"power of two"),
+    (dict(pages=0), _capi.FA2_ERR_INVALID_ARG, b"positive"),
+    (dict(k=0x10008), _capi.FA2_ERR_UNSUPPORTED, b"16-byte"),
+    (dict(v=None), _capi.FA2_ERR_INVALID_ARG, b"non-null"),
+    (dict(k_stride_t=100), _capi.FA2_ERR_UNSUPPORTED, b"multiples of 8"),
+    (dict(v_stride_h=-64), _capi.FA2_ERR_INVALID_ARG, b"negative"),
+    (dict(slot_map=0x10004), _capi.FA2_ERR_INVALID_ARG, b"8-byte"),
+])
+def test_cache_write_refusals(change, code, word):
+    a = _capi.PagedWriteParams()
+    a.k = a.v = a.slot_map = 0x10000
+    a.k_stride_t = a.v_stride_t = 128
+    a.k_stride_h = a.v_stride_h = 64
+    _set_cache(a.k_cache)
+    _set_cache(a.v_cache)
+    a.tokens, a.heads, a.head_dim, a.pages, a.page_size = 5, 2, 64, 7, 16
+    for name, x in change.items():
+        setattr(a, name, x)
+    lib = _capi.load()
+    assert lib.fa2_paged_cache_write(C.byref(a), None) == code
+    assert word in lib.fa2_last_error()
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(head_dim=256), _capi.FA2_ERR_UNSUPPORTED, b"head_dim"),
+    (dict(head_dim=72), _capi.FA2_ERR_UNSUPPORTED, b"head_dim"),
+    (dict(dtype=_capi.FA2_FP32), _capi.FA2_ERR_UNSUPPORTED, b"fp16 and bf16"),
+    (dict(heads_q=5), _capi.FA2_ERR_INVALID_ARG, b"divisible"),
+    (dict(page_size=48), _capi.FA2_ERR_UNSUPPORTED, b"power of two"),
+    (dict(softmax_scale=0.0), _capi.FA2_ERR_INVALID_ARG, b"softmax_scale"),
+    (dict(softmax_scale=math.inf), _capi.FA2_ERR_INVALID_ARG, b"softmax_scale"),
+    (dict(softcap=-1.0), _capi.FA2_ERR_INVALID_ARG, b"softcap"),
+    (dict(q=None), _capi.FA2_ERR_INVALID_ARG, b"non-null"),
+    (dict(o=0x10008), _capi.FA2_ERR_UNSUPPORTED, b"16-byte"),
+    (dict(q_stride_t=4), _capi.FA2_ERR_UNSUPPORTED, b"multiples of 8"),
+    (dict(o_stride_h=0), _capi.FA2_ERR_INVALID_ARG, b"positive"),
+    (dict(table_stride=2), _capi.FA2_ERR_INVALID_ARG, b"table_stride"),
+    (dict(work=0x10004), _capi.FA2_ERR_INVALID_ARG, b"16-byte"),
+    (dict(requests=0), _capi.FA2_ERR_INVALID_ARG, b"positive"),
+])
+def test_paged_attention_refusals(change, code, word):
+    a = _capi.PagedAttentionParams()
+    for name in ("q", "o", "block_table", "work", "workspace"):
+        setattr(a, name, 0x10000)
+    a.q_stride_t = a.o_stride_t = 256
+    a.q_stride_h = a.o_stride_h = 64
+    _set_cache(a.k_cache)
+    _set_cache(a.v_cache)
+    a.tokens, a.heads_q, a.heads_kv, a.head_dim, a.dtype, a.pages, a.page_size = 5, 4, 2, 64, _capi.FA2_BF16, 7, 16
+    a.table_width, a.table_stride, a.requests, a.softmax_scale = 3, 3, 2, 0.1
+    for name, x in change.items():
+        setattr(a, name, x)
+    lib = _capi.load()
+    assert lib.fa2_paged_attention(C.byref(a), None) == code
+    assert word in lib.fa2_last_error()
+
+
+def test_paged_python_layer_refuses_before_any_launch():
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        J.paged_step_plan(ints(2), ints(2), ints(2, 4), ints(3), page_size=16, num_tokens=2, heads_q=4, heads_kv=2)
+    cache = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        J.paged_cache_write(cache[0], cache[0], cache, cache, torch.zeros(16, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        J.paged_attention(cache[0], cache, cache, None)
+    with pytest.raises(ValueError, match="power of two"):
+        J._paged._check_pages(24)
+    with pytest.raises(ValueError, match="same shape"):
+        J._paged._check_caches(cache, cache[:2])
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        J._paged._check_caches(cache.float(), cache.float())
