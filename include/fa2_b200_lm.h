@@ -35,6 +35,11 @@ typedef struct {
   const float* alibi_slopes;   /* float32 [heads_q] on the device, or NULL; takes no gradient    */
   const int32_t* prefix_lens;  /* int32 [batch] on the device, or NULL; needs causal             */
   const int32_t* document_layout;   /* what fa2_document_layout wrote, or NULL; needs Sq == Sk   */
+  /* [batch, seqlen_q, heads_q, head_dim] in the q dtype, or NULL: the forward writes there what rounding o
+   * to 16 bits dropped, the backward adds it to o where it forms rowsum(o * d_o). In bf16 that rounding is
+   * the largest part of the gradients' error where single keys dominate; fp16 does not need it.         */
+  void* o_rest;
+  fa2_strides o_rest_strides;
 } fa2_score_mod;
 
 /* Bytes of the layout of `batch` rows of `seqlen` document ids. */

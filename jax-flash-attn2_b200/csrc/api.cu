@@ -376,6 +376,18 @@ int make_score_mod(ScoreModDev* out, int* mode, const fa2_score_mod& m, const fa
     out->tile_lo = out->tok_hi + tokens;
     out->tile_hi = out->tile_lo + tiles;
   }
+  if (m.o_rest) {
+    if (reinterpret_cast<uintptr_t>(m.o_rest) & 15) return fail(FA2_ERR_UNSUPPORTED, "o_rest must be 16-byte aligned");
+    if ((m.o_rest_strides.b % 8) || (m.o_rest_strides.s % 8) || (m.o_rest_strides.h % 8))
+      return fail(FA2_ERR_UNSUPPORTED, "o_rest: strides must be multiples of 8 elements");
+    HeadDim hd;
+    split_head_dim(p.head_dim, &hd);
+    out->rest = static_cast<uint16_t*>(m.o_rest);
+    out->rest_sb = m.o_rest_strides.b;
+    out->rest_ss = m.o_rest_strides.s;
+    out->rest_sh = m.o_rest_strides.h;
+    out->rest_blk = hd.blk;
+  }
   return FA2_OK;
 }
 
@@ -932,6 +944,10 @@ int fwd_impl(const fa2_fwd_params* a, const fa2_score_mod* mod, void* cuda_strea
     c.d_blk = hd.blk;
     c.sq_pad = sq_pad;
     c.bf16 = bf16;
+    if (mod) {
+      c.rest = mod_dev.rest;
+      c.rest_strides[0] = mod_dev.rest_sb; c.rest_strides[1] = mod_dev.rest_ss; c.rest_strides[2] = mod_dev.rest_sh;
+    }
     e = launch_fwd_combine(c, static_cast<cudaStream_t>(cuda_stream));
     if (e != cudaSuccess)
       return fail(FA2_ERR_CUDA, "split-KV merge launch failed: %s", cudaGetErrorString(e));

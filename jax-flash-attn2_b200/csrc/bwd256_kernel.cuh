@@ -703,7 +703,8 @@ static cudaError_t launch256_passes(const BwdLaunch& a, cudaStream_t stream, Mai
       static_cast<const uint16_t*>(a.o), static_cast<const uint16_t*>(a.d_o), a.o_strides[0],
       a.o_strides[1], a.o_strides[2], a.do_strides[0], a.do_strides[1], a.do_strides[2], kp.lse,
       kp.lse_sb, kp.lse_sh, a.delta, kp.dq_acc, kp.Sq, kp.Hq, nQ128, kBf16 ? nullptr : absmax,
-      a.head_dim_real, kp.seqlens, nullptr, 0.f, kp.dq_order, 4);
+      a.head_dim_real, kp.seqlens, nullptr, 0.f, kp.dq_order, 4, kp.mod.rest, kp.mod.rest_sb, kp.mod.rest_ss,
+      kp.mod.rest_sh);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   mark(1);

@@ -203,7 +203,8 @@ bwd_pre_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ d_o,
                float* __restrict__ stats, float* __restrict__ dq_acc, int Sq, int Hq, int nQ,
                unsigned* __restrict__ do_absmax_bits, int d_real,
                const int* __restrict__ seqlens, uint4* __restrict__ xstats, float inv_scale_log2,
-               int* __restrict__ dq_order, int order_per_tile) {
+               int* __restrict__ dq_order, int order_per_tile, const uint16_t* __restrict__ rest, long long rest_sb,
+               long long rest_ss, long long rest_sh) {
   // one-dimensional grid (the y and z extents of a grid stop at 65535): tile index fastest
   const int i = blockIdx.x % nQ;
   const int bh = blockIdx.x / nQ;
@@ -224,13 +225,20 @@ bwd_pre_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ d_o,
     if (row < sq_b && 8 * sub < d_real) {   // d_real < D: the head dim is padded, rows are d_real wide
       const uint4 a = __ldg(reinterpret_cast<const uint4*>(o + b * o_sb + row * o_ss + h * o_sh) + sub);
       const uint4 g = __ldg(reinterpret_cast<const uint4*>(d_o + b * do_sb + row * do_ss + h * do_sh) + sub);
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+      const uint4 e = rest != nullptr
+                          ? __ldg(reinterpret_cast<const uint4*>(rest + b * rest_sb + row * rest_ss + h * rest_sh) + sub)
+                          : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w}, ew[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         acc = fmaf(to_float16bit<kBf16>(static_cast<uint16_t>(aw[k] & 0xffff)),
                    to_float16bit<kBf16>(static_cast<uint16_t>(gw[k] & 0xffff)), acc);
         acc = fmaf(to_float16bit<kBf16>(static_cast<uint16_t>(aw[k] >> 16)),
                    to_float16bit<kBf16>(static_cast<uint16_t>(gw[k] >> 16)), acc);
+        if (rest != nullptr) {   // what the rounding of o dropped
+          acc = fmaf(unpack_lo<kBf16>(ew[k]), unpack_lo<kBf16>(gw[k]), acc);
+          acc = fmaf(unpack_hi<kBf16>(ew[k]), unpack_hi<kBf16>(gw[k]), acc);
+        }
         if constexpr (!kBf16) {
           const float g0 = fabsf(to_float16bit<kBf16>(static_cast<uint16_t>(gw[k] & 0xffff)));
           const float g1 = fabsf(to_float16bit<kBf16>(static_cast<uint16_t>(gw[k] >> 16)));

@@ -249,6 +249,7 @@ fwd256_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const float sc = kMod > 0 ? 1.f : kFeat ? fs.sc : p.scale_log2;
     const bool prescale = kFeat && fs.prescale;
     float m = -INFINITY, l = 0.f;
+    float l16 = 0.f;       // scored bf16 kernels: the sum of the weights rounded to 16 bits
     bool ok = true;
     // dropout keep bits of this row: those of tile j + 1 are drawn after P of tile j has gone out
     const bool drop_on = kFeat && p.drop.enabled;
@@ -278,9 +279,9 @@ fwd256_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       };
       if constexpr (kScored) {
         const ModTerms<kMod> terms{p.scale_log2, p.mod.cap2, p.mod.arg2, slope2, qi + p.causal_off};
-        softmax_tile_row<kD, kBf16, false, true>(tS, tO, j0 + j, j > 0, p, key_hi_row - 1, sc, false, m, l, wait_pv,
-                                                 [&](int half) { mbar_arrive(bar_p_full(buf, half)); }, terms, keep,
-                                                 key_lo_row);
+        softmax_tile_row<kD, kBf16, false, true, kBf16>(tS, tO, j0 + j, j > 0, p, key_hi_row - 1, sc, false, m, l,
+                                                        wait_pv, [&](int half) { mbar_arrive(bar_p_full(buf, half)); },
+                                                        terms, keep, key_lo_row, &l16);
       } else {
         softmax_tile_row<kD, kBf16, kFeat>(tS, tO, j0 + j, j > 0, p, row_lim, sc, prescale, m, l, wait_pv,
                                            [&](int half) { mbar_arrive(bar_p_full(buf, half)); },
@@ -294,7 +295,9 @@ fwd256_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     if (ok && nt > 0) ok = mbar_wait(bar_o_full, 0, abort_flag);
     if (ok) {
       tc_fence_after();
-      epilogue_row<kD, kBf16, kFeat>(tO, nt > 0, smem_gen + L::kQOff, r, p, b_out, h, qi, sc, m, l);
+      epilogue_row<kD, kBf16, kFeat>(tO, nt > 0, smem_gen + L::kQOff, r, p, b_out, h, qi, sc, m, l,
+                                       kScored && kBf16 ? l16 : l,
+                                       kScored && p.mod.rest && qi < p.Sq ? rest_row(p.mod, b, h, qi) : nullptr);
     }
     named_bar_sync(1, kBM);
     if (ok && r == 0 && !*abort_flag && !p.part_o) {

@@ -15,7 +15,8 @@ __global__ void __launch_bounds__(128)
 fwd_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
                    uint16_t* __restrict__ o, long long osb, long long oss, long long osh,
                    float* __restrict__ lse, long long lse_sb, long long lse_sh, long long lse_sq,
-                   int n_splits, int B, int Sq, int Hq, int D, int D_part, int d_blk, int sq_pad) {
+                   int n_splits, int B, int Sq, int Hq, int D, int D_part, int d_blk, int sq_pad,
+                   uint16_t* __restrict__ rest, long long rsb, long long rss, long long rsh) {
   // one-dimensional grid (the y and z extents of a grid stop at 65535): row fastest, then head
   const int s = blockIdx.x % Sq;
   const int h = (blockIdx.x / Sq) % Hq;
@@ -41,7 +42,10 @@ fwd_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ p
     if (m > -INFINITY)
       for (int k = 0; k < n_splits; ++k)
         acc += __expf(pl[k * lse_split] - total) * po[k * o_split + col];
-    dst[d] = static_cast<uint16_t>(pack2<kBf16>(acc, 0.f) & 0xffffu);
+    const uint32_t v = pack2<kBf16>(acc, 0.f);
+    dst[d] = static_cast<uint16_t>(v & 0xffffu);
+    if (rest)   // what the rounding dropped
+      rest[b * rsb + s * rss + h * rsh + d] = static_cast<uint16_t>(pack2<kBf16>(acc - unpack_lo<kBf16>(v), 0.f) & 0xffffu);
   }
 }
 
@@ -51,12 +55,12 @@ cudaError_t launch_fwd_combine(const FwdCombine& c, cudaStream_t stream) {
     fwd_combine_kernel<true><<<grid, 128, 0, stream>>>(
         c.part_o, c.part_lse, static_cast<uint16_t*>(c.o), c.o_strides[0],
         c.o_strides[1], c.o_strides[2], c.lse, c.lse_sb, c.lse_sh, c.lse_sq, c.n_splits, c.B, c.Sq, c.Hq,
-        c.D, c.D_part, c.d_blk, c.sq_pad);
+        c.D, c.D_part, c.d_blk, c.sq_pad, c.rest, c.rest_strides[0], c.rest_strides[1], c.rest_strides[2]);
   else
     fwd_combine_kernel<false><<<grid, 128, 0, stream>>>(
         c.part_o, c.part_lse, static_cast<uint16_t*>(c.o), c.o_strides[0],
         c.o_strides[1], c.o_strides[2], c.lse, c.lse_sb, c.lse_sh, c.lse_sq, c.n_splits, c.B, c.Sq, c.Hq,
-        c.D, c.D_part, c.d_blk, c.sq_pad);
+        c.D, c.D_part, c.d_blk, c.sq_pad, c.rest, c.rest_strides[0], c.rest_strides[1], c.rest_strides[2]);
   return cudaGetLastError();
 }
 

@@ -411,6 +411,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           qi < it.sq ? (kCausal ? min(it.sk - 1, qi + p.causal_off) : it.sk - 1) : -1;
       float m = -INFINITY;   // running (possibly stale) row maximum, in the units of x[]
       float l = 0.f;         // running row sum of exp2(x*sc - m*sc)
+      float l16 = 0.f;       // scored bf16 kernels: the same of the weights rounded to 16 bits
 
       // keep bits of this row for the tile about to be processed; those of tile j + 1 are drawn
       // after P of tile j has been handed over
@@ -493,8 +494,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
           ok = mbar_wait(bar_s_full(t), it_cnt & 1u, abort_flag);
           if (!ok) break;
-          softmax_tile_row<D, kBf16, false, true>(tS, tO, it.j0 + j, j > 0, p, hi - 1, sc, false, m, l, [] {},
-                                                  [&](int hh) { mbar_arrive(bar_p_full(t, hh)); }, terms, keep, lo);
+          softmax_tile_row<D, kBf16, false, true, kBf16>(tS, tO, it.j0 + j, j > 0, p, hi - 1, sc, false, m, l, [] {},
+                                                         [&](int hh) { mbar_arrive(bar_p_full(t, hh)); }, terms, keep,
+                                                         lo, &l16);
         }
       } else {
         for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
@@ -513,7 +515,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       ++o_cnt;
       // One 64-column block at a time through this tile's 16 KiB staging block. O_t is handed
       // back to the MMA warp as soon as its last columns have been read out of tensor memory.
-      const float inv = (ok && tile_valid) ? epilogue_stats<kFeat>(p, b_out, h, qi, sc, m, l) : 0.f;
+      const float inv = (ok && tile_valid) ? epilogue_stats<kFeat>(p, b_out, h, qi, sc, m, l, kScored && kBf16 ? l16 : l)
+                                           : 0.f;
       uint8_t* stage_gen = smem_gen + L::kOOff + t * L::kBlockBytes;
       tc_fence_after();
 #pragma unroll
@@ -539,6 +542,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
             if (qi < p.Sq) store_partial_row(partial_row<D>(p, b_out, h, qi) + blk * 64, o, inv);
           } else {
             epilogue_block<kBf16>(o, stage_gen, r, inv);
+            if (kScored && p.mod.rest && qi < p.Sq)
+              store_rest<kBf16>(rest_row(p.mod, b, h, qi) + blk * p.mod.rest_blk, 0, p.mod.rest_blk, o, inv);
             fence_proxy_async_smem();
           }
         }

@@ -36,6 +36,8 @@ struct FwdCombine {
   int n_splits, B, Sq, Hq, D, sq_pad;
   int D_part;                 // row length of part_o: the kernel's (padded) head dim
   int d_blk;                  // real columns in each 64-column block of a part_o row
+  uint16_t* rest;             // ScoreModDev::rest with its strides, or null
+  long long rest_strides[3];
   bool bf16;
 };
 cudaError_t launch_fwd_combine(const FwdCombine& c, cudaStream_t stream);

@@ -141,6 +141,8 @@ class ScoreMod(C.Structure):
         ("alibi_slopes", C.c_void_p),
         ("prefix_lens", C.c_void_p),
         ("document_layout", C.c_void_p),
+        ("o_rest", C.c_void_p),
+        ("o_rest_strides", Strides),
     ]
 
 

@@ -70,7 +70,7 @@ def document_layout(document_ids: torch.Tensor) -> torch.Tensor:
     return layout
 
 
-def _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens):
+def _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest=None):
     """(parameter block, tensors kept alive)."""
     mod = _capi.ScoreMod()
     batch, sq, heads = q.shape[:3]
@@ -95,6 +95,10 @@ def _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens):
             raise ValueError("layout must be what document_layout returned for ids of shape "
                              f"[{batch}, {sq}] on the device of q")
         mod.document_layout = layout.data_ptr()
+    if rest is not None:
+        if rest.shape != q.shape or rest.dtype != q.dtype or rest.device != q.device or not rest.is_contiguous():
+            raise ValueError("rest must be a contiguous tensor of the shape, dtype and device of q")
+        mod.o_rest, mod.o_rest_strides = rest.data_ptr(), _strides(rest)
     return mod, (slopes, prefix_lens, layout)
 
 
@@ -109,14 +113,16 @@ def fwd_scored_attention_kernel_call(
     alibi_slopes: tp.Optional[torch.Tensor] = None,
     layout: tp.Optional[torch.Tensor] = None,
     prefix_lens: tp.Optional[torch.Tensor] = None,
+    rest: tp.Optional[torch.Tensor] = None,
 ) -> tp.Tuple[torch.Tensor, torch.Tensor]:
-    """Forward launch; q [B,Sq,Hq,D], k and v [B,Sk,Hkv,D], `layout` from `document_layout`. Returns (out in q.dtype,
+    """Forward launch; q [B,Sq,Hq,D], k and v [B,Sk,Hkv,D], `layout` from `document_layout`. `rest` (a contiguous tensor
+    like q) receives what the rounding of the output dropped, for the backward call. Returns (out in q.dtype,
     lse float32 [B,Hq,ceil(Sq/128)*128] of the changed scores, natural log; columns >= Sq are not written)."""
     _check_qkv(q, k, v)
     lib = _capi.load()
     q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
     batch, sq, hq, d = q.shape
-    mod, _keep = _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens)
+    mod, _keep = _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest)
     out = torch.empty((batch, sq, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((batch, hq, (sq + 127) // 128 * 128), dtype=torch.float32, device=q.device)
     a = _capi.FwdParams()
@@ -148,9 +154,10 @@ def bwd_scored_attention_kernel_call(
     alibi_slopes: tp.Optional[torch.Tensor] = None,
     layout: tp.Optional[torch.Tensor] = None,
     prefix_lens: tp.Optional[torch.Tensor] = None,
+    rest: tp.Optional[torch.Tensor] = None,
     deterministic: tp.Optional[bool] = None,
 ) -> tp.Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Backward launch; `o` and `M` are the forward's output and lse. Returns (dq, dk, dv) in the input dtype. dk and dv
+    """Backward launch; `o`, `M` and `rest` (if it was given) are the forward's output, lse and rest. Returns (dq, dk, dv) in the input dtype. dk and dv
     are the same bits from call to call; dq is so with `deterministic=True` (default None: the environment variable
     FA2_B200_DETERMINISTIC decides, as in `bwd_attention_kernel_call`)."""
     _check_qkv(q, k, v)
@@ -160,7 +167,7 @@ def bwd_scored_attention_kernel_call(
     q, k, v, o, dO = map(_unit_last, (q, k, v, o, dO))
     assert tuple(dO.shape) == tuple(q.shape) and tuple(o.shape) == tuple(q.shape)
     assert dO.dtype == q.dtype and o.dtype == q.dtype
-    mod, _keep = _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens)
+    mod, _keep = _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest)
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
     dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     dv = torch.empty_like(v, memory_format=torch.contiguous_format)
@@ -210,19 +217,24 @@ def _call_with_leaves_noted(operands, call):
 class _ScoredAttentionCall(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, softmax_scale, causal, mods):
-        out, lse = fwd_scored_attention_kernel_call(q, k, v, softmax_scale, causal, **mods)
-        ctx.save_for_backward(q, k, v, out, lse, mods["alibi_slopes"], mods["layout"], mods["prefix_lens"])
+        # bf16: the rounding of the output is the largest error of the gradients where single keys dominate (dq of scores
+        # with a standard deviation of 4 over 100 keys, in float64: 4.6e-3 with it, 3.1e-3 without); what it drops is kept
+        rest = None
+        if q.dtype == torch.bfloat16 and any(ctx.needs_input_grad):
+            rest = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out, lse = fwd_scored_attention_kernel_call(q, k, v, softmax_scale, causal, rest=rest, **mods)
+        ctx.save_for_backward(q, k, v, out, lse, mods["alibi_slopes"], mods["layout"], mods["prefix_lens"], rest)
         ctx.extras = (softmax_scale, causal, mods["softcap"])
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dO):
-        q, k, v, out, lse, slopes, layout, prefix_lens = ctx.saved_tensors
+        q, k, v, out, lse, slopes, layout, prefix_lens, rest = ctx.saved_tensors
         softmax_scale, causal, softcap = ctx.extras
         dq, dk, dv = bwd_scored_attention_kernel_call(
             dO, q, k, v, out, lse, softmax_scale, causal, softcap=softcap, alibi_slopes=slopes, layout=layout,
-            prefix_lens=prefix_lens)
+            prefix_lens=prefix_lens, rest=rest)
         return dq, dk, dv, None, None, None
 
 
