@@ -520,6 +520,7 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         uint32_t s[32];
         tmem_ld32(tS, s);
         tc_wait_ld();
+        if constexpr (has_cap(kMod)) tanh_row(reinterpret_cast<float(&)[32]>(s), p.mod.arg2);
         if constexpr (kFeat) {
 #pragma unroll
           for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) * p.scale_log2);
@@ -536,7 +537,7 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             float x0 = __uint_as_float(s[c]), x1 = __uint_as_float(s[c + 1]);
             float g0 = 1.f, g1 = 1.f;
             if constexpr (kScored) {
-              mod_exponents<kMod>(x0, x1, nlv[2 * k2], nlv[2 * k2 + 1], p.scale_log2, p.mod.cap2, p.mod.arg2, slope2,
+              mod_exponents<kMod>(x0, x1, nlv[2 * k2], nlv[2 * k2 + 1], p.scale_log2, p.mod.cap2, slope2,
                                   static_cast<float>(q_first + p.causal_off - kv) + static_cast<float>(c), g0, g1);
             } else if constexpr (kFeat) {
               x0 += nlv[2 * k2];      // already scaled, bias and mask added (below the loads)

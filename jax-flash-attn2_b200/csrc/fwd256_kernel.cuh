@@ -246,7 +246,7 @@ fwd256_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const uint32_t tO = tmem_base + lane_base + kColO;
     const int row_lim = qi < sq_b ? (kCausal ? min(sk_b - 1, qi + p.causal_off) : sk_b - 1) : -1;
     const FeatScale fs(p.scale_log2);
-    const float sc = kMod > 0 ? 1.f : kFeat ? fs.sc : p.scale_log2;
+    const float sc = kMod > 0 ? ModTerms<kMod>::sc(p.scale_log2, p.mod.cap2) : kFeat ? fs.sc : p.scale_log2;
     const bool prescale = kFeat && fs.prescale;
     float m = -INFINITY, l = 0.f;
     float l16 = 0.f;       // scored bf16 kernels: the sum of the weights rounded to 16 bits
@@ -265,7 +265,7 @@ fwd256_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 
     int key_lo_row = 0, key_hi_row = 0;   // scored kernels: the keys this row sees
     if (kScored && qi < p.Sq) query_interval(p.mod, b, qi, p.Sq, p.Sk, p.causal_off, key_lo_row, key_hi_row);
-    const float slope2 = has_slope(kMod) ? __ldg(p.mod.slopes + h) * kLog2e : 0.f;
+    const float slope_h = has_slope(kMod) ? __ldg(p.mod.slopes + h) : 0.f;
 
     for (int j = 0; j < nt; ++j) {
       const int buf = j & 1;
@@ -278,7 +278,7 @@ fwd256_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         tc_fence_after();
       };
       if constexpr (kScored) {
-        const ModTerms<kMod> terms{p.scale_log2, p.mod.cap2, p.mod.arg2, slope2, qi + p.causal_off};
+        const ModTerms<kMod> terms(p.scale_log2, p.mod.arg2, p.mod.cap2, slope_h, qi + p.causal_off);
         softmax_tile_row<kD, kBf16, false, true, kBf16>(tS, tO, j0 + j, j > 0, p, key_hi_row - 1, sc, false, m, l,
                                                         wait_pv, [&](int half) { mbar_arrive(bar_p_full(buf, half)); },
                                                         terms, keep, key_lo_row, &l16);

@@ -384,7 +384,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     const uint32_t tS = tmem_base + lane_base + kColS + t * kBN;
     const uint32_t tO = tmem_base + lane_base + kColO + t * D;
     const FeatScale fs(p.scale_log2);
-    const float sc = kMod > 0 ? 1.f : kFeat ? fs.sc : p.scale_log2;   // multiplies the values held in x[]
+    const float sc = kMod > 0 ? ModTerms<kMod>::sc(p.scale_log2, p.mod.cap2) : kFeat ? fs.sc : p.scale_log2;   // multiplies the values held in x[]
     const bool prescale = kFeat && fs.prescale;
     uint32_t it_cnt = 0;       // tile-iterations so far: phase of s_full / p_full
     uint32_t o_cnt = 0;        // items so far: phase of o_full
@@ -489,8 +489,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
       } else if constexpr (kScored) {
         int lo = 0, hi = 0;
         if (qi < p.Sq) query_interval(p.mod, b, qi, p.Sq, p.Sk, p.causal_off, lo, hi);
-        const ModTerms<kMod> terms{p.scale_log2, p.mod.cap2, p.mod.arg2,
-                                   has_slope(kMod) ? __ldg(p.mod.slopes + h) * kLog2e : 0.f, qi + p.causal_off};
+        const ModTerms<kMod> terms(p.scale_log2, p.mod.arg2, p.mod.cap2, has_slope(kMod) ? __ldg(p.mod.slopes + h) : 0.f,
+                                   qi + p.causal_off);
         for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
           ok = mbar_wait(bar_s_full(t), it_cnt & 1u, abort_flag);
           if (!ok) break;

@@ -385,7 +385,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem_base + lane_base + kColS + t * kBN;
     const uint32_t tO = tmem_base + lane_base + kColO + t * D;
-    const float sc = kMod > 0 ? 1.f : p.scale_log2;
+    const float sc = ModTerms<kMod>::sc(p.scale_log2, p.cap2);
     const int tok = r / p.G, head = r - tok * p.G;     // this row's token in the tile and head in the group
     FwdKernelParams none;                              // softmax_tile_row reads nothing of it without score terms
     const KeepBitsDropout keep{false, make_uint4(0u, 0u, 0u, 0u)};
@@ -403,8 +403,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const int row_lim = valid ? min(pos, s.seen - 1) : -1;
       const int h = s.hk * p.G + head;
       float m = -INFINITY, l = 0.f;
-      const ModTerms<kMod> terms{p.scale_log2, p.cap2, p.arg2, has_slope(kMod) && valid ? __ldg(p.slopes + h) * kLog2e : 0.f,
-                                 pos};
+      const ModTerms<kMod> terms(p.scale_log2, p.arg2, p.cap2, has_slope(kMod) && valid ? __ldg(p.slopes + h) : 0.f, pos);
       for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
         ok = mbar_wait(bar_s_full(t), it_cnt & 1u, abort_flag);
         if (!ok) break;

@@ -7,10 +7,7 @@
 // of queries that see a key is an interval for the same reason, so a row of a tile needs two compares at most, and
 // whole tiles outside the interval are never loaded.
 //
-// The tanh is 1 - 2 / (e^(2z) + 1) with z = s / cap: one exponential and one reciprocal. Its absolute error is about
-// 2^-22, which cap * log2(e) turns into an error of the exponent below 2^-21 * cap (3e-5 at a cap of 50): far below
-// the 2^-9 of the rounding of P. The hardware's tanh (2^-11 relative) would move the weights by a percent there. The
-// derivative 1 - tanh^2 is 4 r (1 - r) with the same reciprocal r, without a cancellation where tanh is near 1.
+// With t = tanh(s / cap) the derivative of a capped score is 1 - t^2.
 #pragma once
 #include "kernel_params.cuh"
 #include "ptx_sm100.cuh"
@@ -25,6 +22,7 @@ constexpr int kModSlope = 2;
 constexpr bool has_cap(int mod) { return mod > 0 && (mod & kModCap); }
 constexpr bool has_slope(int mod) { return mod > 0 && (mod & kModSlope); }
 
+constexpr float kLog2eMod = 1.4426950408889634f;
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -122,61 +120,101 @@ __device__ __forceinline__ int key_tiles_above(const ScoreModDev& m, int b, int 
   return count;
 }
 
-// The forward's score change of one query row and 128 keys from kv0: x holds the dot products and becomes the scores
-// in units of log2 (left alone without a cap and slopes: the softmax then scales them itself).
+// tanh(z) of N values of a row, z = ln2 / 2 * arg2 * x (that is, e^(2z) = 2^(arg2 x)), in place. All 32 lanes call it.
+//
+// Where every |z| of the warp's values is at most 1 (scores below the cap, which is what a cap is chosen for), it is an odd
+// polynomial, z times a polynomial of degree 5 in z^2 that is best in the maximum norm (found by weighted least squares
+// repeated until the error levels out): |error| <= 2.4e-7, fused multiply-adds of pairs alone. Otherwise 1 - 2 r with
+// r = 1 / (1 + 2^(arg2 x)): an exponential and a reciprocal, |error| <= 2^-22. A cap of 50 turns either into at most 2^-15
+// in the exponent of a weight, far below the 2^-9 of the rounding of P; the hardware's tanh (2^-11 relative) would move the
+// weights by percents. The special functions are what a capped kernel would be bound by otherwise: 16 lanes per cycle and SM,
+// three per score. Measured (2 x 8192 causal, 32/8 heads, D = 128, cap 50): forward 1.96 ms with the second form alone,
+// 2.00 with a polynomial in 2^-|arg2 x| instead of the reciprocal, 1.70 ms as it is; backward 3.61, 3.84, 3.54 ms.
+constexpr float kSmallTanh = 2.8853900817779268f;   // 2 log2(e): |arg2 x| at |z| = 1
+constexpr float kT0 = 0.34657249991665245f, kT1 = -0.013872143458246167f, kT2 = 0.0006626874361558277f,
+                kT3 = -3.061309816091965e-05f, kT4 = 1.1624315928559195e-06f, kT5 = -2.4602920433007444e-08f;
+template <int N>
+__device__ __forceinline__ void tanh_row(float (&x)[N], float arg2) {
+  float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < N; c += 4) {
+    a0 = max3(a0, fabsf(x[c]), fabsf(x[c + 1]));
+    a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
+  }
+  if (!__any_sync(0xffffffffu, fmaxf(a0, a1) * arg2 > kSmallTanh)) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      float y0, y1, u0, u1, t0, t1;
+      fma2(y0, y1, x[c], x[c + 1], arg2, arg2, 0.f, 0.f);
+      fma2(u0, u1, y0, y1, y0, y1, 0.f, 0.f);
+      fma2(t0, t1, u0, u1, kT5, kT5, kT4, kT4);
+      fma2(t0, t1, t0, t1, u0, u1, kT3, kT3);
+      fma2(t0, t1, t0, t1, u0, u1, kT2, kT2);
+      fma2(t0, t1, t0, t1, u0, u1, kT1, kT1);
+      fma2(t0, t1, t0, t1, u0, u1, kT0, kT0);
+      fma2(x[c], x[c + 1], t0, t1, y0, y1, 0.f, 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      fma2(x[c], x[c + 1], x[c], x[c + 1], arg2, arg2, 0.f, 0.f);
+      const float r0 = rcp_approx(1.f + ex2_approx(x[c])), r1 = rcp_approx(1.f + ex2_approx(x[c + 1]));
+      fma2(x[c], x[c + 1], r0, r1, -2.f, -2.f, 1.f, 1.f);
+    }
+  }
+}
+
+// The forward's score change of one query row and 128 keys from kv0: x holds the dot products and becomes the scores,
+// which the softmax multiplies by `sc` to get units of log2: tanh(s / cap) with sc = cap * log2(e), with slopes alone the
+// scores in units of log2 with sc = 1, without either the dot products with sc = softmax_scale * log2(e).
 template <int kMod>
 struct ModTerms {
-  float scale_log2, cap2, arg2;
-  float slope2;     // slope_h * log2(e)
+  float scale_log2, arg2;
+  float slope;      // slope_h * log2(e) / sc
   int qpos;         // position of the query among the keys: i + Sk - Sq
+  __device__ __forceinline__ ModTerms(float scale_log2_, float arg2_, float cap2, float slope_h, int qpos_)
+      : scale_log2(scale_log2_), arg2(arg2_), slope(slope_h * kLog2eMod), qpos(qpos_) {
+    if constexpr (has_cap(kMod)) slope *= 1.f / cap2;
+  }
+  static __device__ __forceinline__ float sc(float scale_log2, float cap2) {
+    return has_cap(kMod) ? cap2 : has_slope(kMod) ? 1.f : scale_log2;
+  }
   template <int N>
   __device__ __forceinline__ void operator()(float (&x)[N], int kv0) const {
-    if constexpr (has_cap(kMod)) {
-      const float c2 = -2.f * cap2;
-#pragma unroll
-      for (int c = 0; c < N; c += 2) {
-        const float r0 = rcp_approx(1.f + ex2_approx(x[c] * arg2));
-        const float r1 = rcp_approx(1.f + ex2_approx(x[c + 1] * arg2));
-        fma2(x[c], x[c + 1], r0, r1, c2, c2, cap2, cap2);
-      }
-    }
+    if constexpr (has_cap(kMod)) tanh_row(x, arg2);
     if constexpr (has_slope(kMod)) {
       const float mul = has_cap(kMod) ? 1.f : scale_log2;
       const float base = static_cast<float>(kv0 - qpos);
       if (kv0 + N - 1 <= qpos || kv0 >= qpos) {
         // all keys on one side of the query: the bias is linear in the key
-        const float s = kv0 >= qpos ? -slope2 : slope2;
+        const float s = kv0 >= qpos ? -slope : slope;
         float b0 = base, b1 = base + 1.f;
 #pragma unroll
         for (int c = 0; c < N; c += 2) {
           float t0, t1;
-          fma2(x[c], x[c + 1], x[c], x[c + 1], mul, mul, 0.f, 0.f);
+          if constexpr (!has_cap(kMod)) fma2(x[c], x[c + 1], x[c], x[c + 1], mul, mul, 0.f, 0.f);
           add2(t0, t1, b0, b1, static_cast<float>(c), static_cast<float>(c));
           fma2(x[c], x[c + 1], t0, t1, s, s, x[c], x[c + 1]);
         }
       } else {
 #pragma unroll
         for (int c = 0; c < N; ++c)
-          x[c] = fmaf(fabsf(base + static_cast<float>(c)), -slope2, x[c] * mul);
+          x[c] = fmaf(fabsf(base + static_cast<float>(c)), -slope, x[c] * mul);
       }
     }
   }
 };
 
 // The backward's score change of two entries of a key row: s0 and s1 hold the dot products (or, where the row
-// statistics are folded into them, the dot products minus lse / scale) and become the exponents of P in units of
-// log2, up to the statistics n0 and n1 (-lse * log2(e)); g0 and g1 receive d score / d (scale * dot product).
-// d0: position of the first entry's query minus the key's.
+// statistics are folded into them, the dot products minus lse / scale; with a cap tanh_row's results) and become the
+// exponents of P in units of log2, up to the statistics n0 and n1 (-lse * log2(e)); g0 and g1 receive
+// d score / d (scale * dot product). d0: position of the first entry's query minus the key's.
 template <int kMod>
 __device__ __forceinline__ void mod_exponents(float& s0, float& s1, float n0, float n1, float scale_log2, float cap2,
-                                              float arg2, float slope2, float d0, float& g0, float& g1) {
+                                              float slope2, float d0, float& g0, float& g1) {
   if constexpr (has_cap(kMod)) {
-    const float r0 = rcp_approx(1.f + ex2_approx(s0 * arg2)), r1 = rcp_approx(1.f + ex2_approx(s1 * arg2));
-    float t0, t1;
-    fma2(t0, t1, r0, r1, -4.f, -4.f, 4.f, 4.f);     // 4 (1 - r)
-    fma2(g0, g1, t0, t1, r0, r1, 0.f, 0.f);         // 1 - tanh^2 = 4 r (1 - r)
-    add2(n0, n1, n0, n1, cap2, cap2);
-    fma2(s0, s1, r0, r1, -2.f * cap2, -2.f * cap2, n0, n1);
+    fma2(g0, g1, s0, s1, -s0, -s1, 1.f, 1.f);
+    fma2(s0, s1, s0, s1, cap2, cap2, n0, n1);
   } else {
     fma2(s0, s1, s0, s1, scale_log2, scale_log2, n0, n1);
   }

@@ -6,8 +6,8 @@ kernel with 16-bit operands makes on the way, worst case, entry by entry (u: hal
   out is rounded once                                                 err(o)  = err(P) |V| + u |o|
   delta = rowsum(dO * out) uses the rounded out                       err(dl) = sum |dO| err(o)
   dS = P g (dP - delta): P (or P g) is rounded, then dS               err(dS) = 2 u |dS| + P g err(dl) (+ subnormals)
-  a capped score's g = 4 r (1 - r) in float32, r a reciprocal off by at most 2^-23: err(g) = 4 * 2^-23 = 2^-21, and
-  P err(g) |dP - delta| of it reaches dS
+  a capped score's g = 1 - t^2 in float32 with t = 1 - 2 r, r a reciprocal off by at most 2^-23 and the difference by
+  2^-24: err(t) <= 2^-22 + 2^-24, err(g) <= 2 err(t) + 2^-24 < 2^-20, and P err(g) |dP - delta| of it reaches dS
   dq, dk, dv are rounded once
 `slack` covers what float32 loses inside the exponent (products of D terms, the cap's exponential and reciprocal,
 a distance times a slope), as a relative change of P.
@@ -96,7 +96,7 @@ def bounds(r, dtype, slack=5e-4):
         size = do @ r["v"].abs().transpose(-1, -2) + (do * r["o"].abs()).sum(-1, keepdim=True)
         err_ds = (2 * u + slack) * r["ds"].abs() + r["pg"] * (err_delta + 1e-5 * size)
         if r["capped"]:
-            err_ds = err_ds + 2.0 ** -21 * r["p"] * r["inner"].abs()
+            err_ds = err_ds + 2.0 ** -20 * r["p"] * r["inner"].abs()
         if tiny:
             err_ds = err_ds + tiny * size * (r["p"] > 0) + tiny * 2 * do.max() * (r["p"] > 0)
         b["dq"] = (r["scale"] * (err_ds @ r["k"].abs())).permute(0, 2, 1, 3) + u * r["dq"].abs()
