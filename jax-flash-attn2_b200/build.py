@@ -1,7 +1,8 @@
-"""Builds libfa2_b200.so (the C-ABI library with the sm_100a kernels) in-tree with nvcc.
+"""Builds libfa2_b200.so (the C-ABI library with the sm_100a kernels) with nvcc and the Python binding of its operators
+for language models (jax_flash_attn2/_fa2_native.so) with g++, both in-tree.
 
 Usage: python build.py [--force] [--verbose]
-The library is written beside this file so that it travels with the source tree.
+The library is written beside this file, the binding into the package, so that both travel with the source tree.
 """
 from __future__ import annotations
 
@@ -16,6 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "libfa2_b200.so")
+BINDING_SRC = os.path.join(HERE, "binding", "fa2_native.cpp")
+BINDING_PATH = os.path.join(HERE, "jax_flash_attn2", "_fa2_native.so")
 SOURCES = ["api.cu", "fwd_sm100.cu", "fwd256_sm100.cu", "fwd_combine.cu", "bwd_sm100.cu", "bwd256_sm100.cu",
            "fwd_scored64_sm100.cu", "fwd_scored128_sm100.cu", "fwd_scored256_sm100.cu",
            "bwd_scored64_sm100.cu", "bwd_scored128_sm100.cu", "bwd_scored256_sm100.cu", "document_layout.cu",
@@ -58,8 +61,39 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def build_binding(force: bool = False) -> str:
+    """Compiles the binding against the installed torch; returns its path."""
+    newest = max(os.path.getmtime(p) for p in (BINDING_SRC, os.path.join(HERE, "..", "include", "fa2_b200.h"),
+                                               os.path.join(HERE, "..", "include", "fa2_b200_lm.h"), os.path.abspath(__file__)))
+    if not force and os.path.exists(BINDING_PATH) and os.path.getmtime(BINDING_PATH) >= newest:
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in include), BINDING_SRC,
+           "-o", BINDING_PATH, "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda",
+           "-ltorch_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SRC}:\n{res.stdout}\n{res.stderr}")
+    return BINDING_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles every kernel for sm_100a and links the shared library; returns its path."""
+    """Compiles every kernel for sm_100a, links the shared library and builds the binding; returns the library's path."""
+    with concurrent.futures.ThreadPoolExecutor(max_workers=1) as pool:
+        binding = pool.submit(build_binding, force)
+        path = _build_library(force, verbose)
+        binding.result()
+    return path
+
+
+def _build_library(force: bool, verbose: bool) -> str:
     if not force and os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= _newest_input():
         return LIB_PATH
     os.makedirs(OBJ_DIR, exist_ok=True)

@@ -20,12 +20,12 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _capi
+from . import _capi, _native
 from ._kernel_calls import _DTYPE_CODE, _launch
 from ._scored_attention import _check_slopes, _check_softcap
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False)
 class PagedStepPlan:
     """What `paged_step_plan` computed, on the device. `block_table` is the caller's, updated in place."""
 
@@ -79,6 +79,13 @@ def paged_step_plan(
     the same plan: the lengths and the free list are the caller's to advance (`free_start += plan.pages_taken` on the
     device). Where the list runs out (pages_taken says how much was needed), table entries and slots are -1: such tokens
     are not written, and attention reads zeros in their place."""
+    parts = _native.load().paged_step_plan(context_lens, new_lens, block_table, free_pages, page_size, num_tokens, heads_q,
+                                           heads_kv, free_start)
+    if parts is not None:
+        cu_seqlens, seqlens_k, slot_map, positions, pages_taken, work = parts
+        return PagedStepPlan(cu_seqlens, seqlens_k, block_table, slot_map, positions, pages_taken, work, page_size, num_tokens,
+                             heads_q, heads_kv)
+    # the call is to be refused, or some operand has to be copied first
     if not block_table.is_cuda:
         raise RuntimeError("fa2_b200 runs on CUDA tensors only; there is no CPU path")
     page_size, num_tokens = _check_pages(page_size), int(num_tokens)
@@ -141,6 +148,9 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
                       slot_map: torch.Tensor) -> None:
     """Writes row t of k and v ([T, Hkv, D], strided rows and heads allowed) to slot `slot_map[t]` (int64 [T]) of the
     caches [pages, page_size, Hkv, D]. Slots outside the cache (-1) are skipped; no slot may occur twice."""
+    if _native.load().paged_cache_write(k, v, k_cache, v_cache, slot_map):
+        return
+    # the call is to be refused, or some operand has to be copied first
     if not k_cache.is_cuda:
         raise RuntimeError("fa2_b200 runs on CUDA tensors only; there is no CPU path")
     _check_caches(k_cache, v_cache)
@@ -187,6 +197,12 @@ def paged_attention(
     Returns `out` [T, Hq, D] (allocated if not given); rows behind the last request are left as they were. `lse`: float32
     [T, Hq] to be filled with the natural log-sum-exp of the scores. Memory in a request's last page behind its last key
     is ignored whatever it holds. No gradients: inference only."""
+    if isinstance(plan, PagedStepPlan):
+        done = _native.load().paged_attention(q, k_cache, v_cache, plan.block_table, plan.work, plan.num_tokens, plan.heads_q,
+                                              plan.heads_kv, plan.page_size, softmax_scale, softcap, alibi_slopes, out, lse)
+        if done is not None:
+            return done
+    # the call is to be refused, or some operand has to be copied first
     if not q.is_cuda:
         raise RuntimeError("fa2_b200 runs on CUDA tensors only; there is no CPU path")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):

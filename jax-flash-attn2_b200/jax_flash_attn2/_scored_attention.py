@@ -23,7 +23,7 @@ import typing as tp
 
 import torch
 
-from . import _capi
+from . import _capi, _native
 from ._kernel_calls import _check_qkv, _launch, _problem, _strides, _unit_last
 
 
@@ -68,6 +68,11 @@ def document_layout(document_ids: torch.Tensor) -> torch.Tensor:
         _capi.check(lib.fa2_document_layout(document_ids.data_ptr(), document_ids.stride(0), batch, seqlen,
                                             layout.data_ptr(), nbytes, C.c_void_p(stream)))
     return layout
+
+
+def _check_devices(q, k, v):
+    if not (q.device == k.device == v.device):
+        raise ValueError(f"q, k and v must live on one device, got {q.device}, {k.device} and {v.device}")
 
 
 def _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest=None):
@@ -119,6 +124,7 @@ def fwd_scored_attention_kernel_call(
     like q) receives what the rounding of the output dropped, for the backward call. Returns (out in q.dtype,
     lse float32 [B,Hq,ceil(Sq/128)*128] of the changed scores, natural log; columns >= Sq are not written)."""
     _check_qkv(q, k, v)
+    _check_devices(q, k, v)
     lib = _capi.load()
     q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
     batch, sq, hq, d = q.shape
@@ -161,10 +167,13 @@ def bwd_scored_attention_kernel_call(
     are the same bits from call to call; dq is so with `deterministic=True` (default None: the environment variable
     FA2_B200_DETERMINISTIC decides, as in `bwd_attention_kernel_call`)."""
     _check_qkv(q, k, v)
+    _check_devices(q, k, v)
     lib = _capi.load()
     if deterministic is None:
         deterministic = os.environ.get("FA2_B200_DETERMINISTIC", "0") not in ("", "0")
-    q, k, v, o, dO = map(_unit_last, (q, k, v, o, dO))
+    q, k, v, o = map(_unit_last, (q, k, v, o))
+    if dO.stride(-1) != 1 or dO.data_ptr() % 16 or any(s <= 0 or s % 8 for s in dO.stride()[:3]):
+        dO = dO.clone(memory_format=torch.contiguous_format)      # a cotangent may be expanded or transposed
     assert tuple(dO.shape) == tuple(q.shape) and tuple(o.shape) == tuple(q.shape)
     assert dO.dtype == q.dtype and o.dtype == q.dtype
     mod, _keep = _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest)
@@ -192,28 +201,6 @@ def bwd_scored_attention_kernel_call(
     return dq, dk, dv
 
 
-def _leaf_nodes(operands):
-    return [torch.autograd.graph.get_gradient_edge(x).node for x in operands if x.requires_grad and x.is_leaf]
-
-
-def _call_with_leaves_noted(operands, call):
-    """The node that accumulates the gradient of a leaf belongs to the stream it was made on and lives as long as any
-    graph that ends in it. A backward pass captured into a CUDA graph while such a node of another stream lives makes
-    autograd synchronise with that stream, which breaks the capture. So a call of this operator leaves its stream at
-    the node of each leaf, and a call under capture that finds another stream there is refused before anything is
-    spoilt."""
-    stream = torch.cuda.current_stream(operands[0].device).cuda_stream
-    if torch.cuda.is_current_stream_capturing():
-        for node in _leaf_nodes(operands):
-            if node.metadata.get("fa2_b200_stream", stream) != stream:
-                raise RuntimeError("a forward pass on another stream has a live autograd graph with the same leaf tensors: "
-                                   "drop its outputs (or detach them) before capturing this call into a CUDA graph")
-    out = call()
-    for node in _leaf_nodes(operands):      # alive now: the graph behind `out` holds it
-        node.metadata.setdefault("fa2_b200_stream", stream)
-    return out
-
-
 class _ScoredAttentionCall(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, softmax_scale, causal, mods):
@@ -228,8 +215,9 @@ class _ScoredAttentionCall(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dO):
+        if torch.is_grad_enabled():
+            raise RuntimeError("scored_flash_attention has no second derivatives (create_graph=True)")
         q, k, v, out, lse, slopes, layout, prefix_lens, rest = ctx.saved_tensors
         softmax_scale, causal, softcap = ctx.extras
         dq, dk, dv = bwd_scored_attention_kernel_call(
@@ -256,8 +244,17 @@ def scored_flash_attention(
     q [B,Sq,Hq,D]; k, v [B,Sk,Hkv,D] with Hq a multiple of Hkv; fp16 or bf16; the head dims and strides of
     `triton_flash_attention`. softmax_scale (default 1/sqrt(D)) must be positive; softcap lies in [2^-10, 1024];
     alibi_slopes float32 [Hq]; document_ids int32 [B, S] with Sq == Sk == S (or their `layout`, so that several layers
-    share it); prefix_lens int32 [B], with causal=True. All on the device of q. Returns [B,Sq,Hq,D] in q.dtype."""
+    share it); prefix_lens int32 [B], with causal=True. All on the device of q. Returns [B,Sq,Hq,D] in q.dtype.
+
+    The backward pass may be captured into a CUDA graph unless the graph of an earlier call on another stream still lives and
+    ends in the same leaf tensors: autograd would synchronise with that stream, so the call is refused under capture."""
+    out = _native.load().scored_flash_attention(q, k, v, softmax_scale, causal, softcap, alibi_slopes, document_ids,
+                                                prefix_lens, layout)
+    if out is not None:
+        return out
+    # the call is to be refused, or some operand has to be copied first
     _check_qkv(q, k, v)
+    _check_devices(q, k, v)
     if document_ids is not None:
         if layout is not None:
             raise ValueError("give document_ids or their layout, not both")
@@ -269,5 +266,6 @@ def scored_flash_attention(
         layout = document_layout(document_ids)
     mods = dict(softcap=softcap, alibi_slopes=_check_slopes(alibi_slopes, q.shape[2], q.device), layout=layout,
                 prefix_lens=prefix_lens)
-    call = lambda: _ScoredAttentionCall.apply(q, k, v, softmax_scale, bool(causal), mods)
-    return _call_with_leaves_noted((q, k, v), call) if torch.is_grad_enabled() else call()
+    if torch.is_grad_enabled():
+        _native.load().check_capture(q, k, v)
+    return _ScoredAttentionCall.apply(q, k, v, softmax_scale, bool(causal), mods)

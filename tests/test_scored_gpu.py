@@ -266,3 +266,44 @@ def test_without_changes_it_is_the_plain_attention():
     b = J.triton_flash_attention(q, k, v, causal=True).float()
     weight = J.triton_flash_attention(q, k, v.abs(), causal=True).float()
     assert torch.all((a - b).abs() <= 2 * 2.0 ** -8 * (weight + b.abs()))
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_cotangents_of_any_layout(D):
+    """An expanded cotangent (strides of zero), a transposed one and a misaligned one give the dense one's gradients."""
+    import jax_flash_attn2 as J
+    q, k, v, do = (x.cuda() for x in W.make_qkv(2, 130, 130, 4, 2, D, BF16))
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = J.scored_flash_attention(*leaves, None, True, softcap=20.0)
+    grads = lambda c: torch.autograd.grad(out, leaves, c, retain_graph=True)
+    one = torch.full_like(do, 0.5)
+    for got, want in ((grads(one[:1, :1, :1, :1].expand_as(one)), grads(one)),
+                      (grads(do.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)), grads(do)),
+                      (grads(torch.cat([do.flatten()[:1], do.flatten()])[1:].view_as(do)), grads(do))):
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(out, leaves, do, create_graph=True)
+
+
+def test_some_operands_without_gradients_and_operands_to_be_copied():
+    import jax_flash_attn2 as J
+    q, k, v, do = (x.cuda() for x in W.make_qkv(1, 100, 100, 2, 2, 64, BF16))
+    full = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    want = torch.autograd.grad(J.scored_flash_attention(*full, None, True, softcap=20.0), full, do)
+    k2 = k.clone().requires_grad_(True)
+    got = torch.autograd.grad(J.scored_flash_attention(q, k2, v, None, True, softcap=20.0), k2, do)
+    assert torch.equal(got[0], want[1])
+    # columns that do not lie next to each other are copied before the launch
+    odd = [x.transpose(2, 3).contiguous().transpose(2, 3).requires_grad_(True) for x in (q, k, v)]
+    assert odd[0].stride(3) != 1
+    out = J.scored_flash_attention(*odd, None, True, softcap=20.0)
+    again = torch.autograd.grad(out, odd, do)
+    assert torch.equal(again[1], want[1]) and torch.equal(again[2], want[2])
+    with torch.no_grad():
+        assert torch.equal(J.scored_flash_attention(*full, None, True, softcap=20.0), out)
+    with pytest.raises(J._capi.Fa2Error, match="head_dim"):
+        J.scored_flash_attention(*(torch.zeros(1, 8, 2, 72, dtype=BF16, device="cuda") for _ in range(3)))
+    with pytest.raises(ValueError, match="softcap"):
+        J.scored_flash_attention(q, k, v, softcap=-1.0)
+    with pytest.raises(AssertionError, match="fp16 and bf16"):
+        J.scored_flash_attention(q.float(), k.float(), v.float())
