@@ -9,9 +9,9 @@ namespace fa2 {
 
 cudaError_t launch_document_layout(const int* ids, long long stride_b, int B, int S, int* layout, cudaStream_t stream);
 
-// Work list of the paged attention (int32): a header of kWorkHeader words (0: items, 1: key tiles of all items
-// together), then kWorkItem words per item: first row of the packed tensors, tokens, position of the first token,
-// request, key tiles of the items before it, key tiles of its own, 0, 0.
+// Work list of the paged attention (int32): a header of kWorkHeader words (0: items, 1: cost of all items together),
+// then kWorkItem words per item: first row of the packed tensors, tokens, position of the first token, request, cost of
+// the items before it, key tiles of its own, cost of a key tile (1 or 2), 0.
 constexpr int kWorkHeader = 16;
 constexpr int kWorkItem = 8;
 

@@ -7,11 +7,18 @@
 // read once per group: a 128-row tile holds floor(128 / G) tokens, an item (two tiles over one stream of keys, as in
 // fwd_kernel.cuh) twice as many.
 //
-// Split. The key tiles of all items of all key/value heads are numbered through, W in all, and CTA c works on the tiles
-// [c W / n, (c + 1) W / n): every SM streams the same number of tiles whatever the lengths of the requests are. A CTA that
-// has all key tiles of an item writes its rows; items cut by a border leave normalised partial rows and their log-sum-exp in
+// Split. The key tiles of all items of all key/value heads stand on one line, W long in all, on which a tile of a two-tile item
+// takes 2 and one of a smaller item 1 (what they cost: see "Few rows"), and CTA c works on the tiles that begin in
+// [c W / n, (c + 1) W / n): every SM gets the same share whatever the lengths of the requests are. A CTA that has all key
+// tiles of an item writes its rows; items cut by a border leave normalised partial rows and their log-sum-exp in
 // float32 (at most two per CTA), which paged_combine_kernel joins in the order of the keys: the result does not depend on
 // which CTA was faster.
+//
+// Few rows. An item whose tokens fit one query tile (every single token) is bound by the chain S -> softmax -> P V of a key
+// tile, not by its work. It runs as two chains: the second warpgroup takes the odd key tiles of the same rows, with its own
+// maximum, sum and accumulator, and the first one joins the two accumulators when it writes the rows, straight from tensor
+// memory (the rows lie on the same lanes). 64 decodes over 128 .. 16384 keys (32/8 heads, D = 128): 161 us with one chain,
+// DUAL us with two; the cache alone is 646 MB, 98 us at the measured copy bandwidth.
 //
 // Keys. Pages hold 2^s tokens; a 128-key tile takes 128 / 2^s pieces of a page each (one if pages are larger), every piece
 // and 64-column block one TMA box, issued by a lane of its own. Pages outside the request or the pool are fetched from
@@ -38,7 +45,7 @@ template <int D>
 struct PagedSmem {
   static constexpr int kQTileBytes = 128 * D * 2;
   static constexpr int kKVTileBytes = 128 * D * 2;
-  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr int kStages = D == 64 ? 10 : 5;
   static constexpr int kBlock = 128 * 128;             // one [128 rows][64 elements] block
   static constexpr int kQOff = 0;
   static constexpr int kKVOff = kQOff + 2 * kQTileBytes;
@@ -46,16 +53,18 @@ struct PagedSmem {
   // q_full[2], q_free[2], kv_full[S], kv_empty[S], s_full[2], p_full[2][kPSplit], o_full[2], o_free[2], dirty, clean
   static constexpr int kNumBars = 4 + 2 * kStages + 2 + 2 * kPSplit + 4 + 2;
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kTotal = kMiscOff + 16;
+  static constexpr int kStatOff = kMiscOff + 16;       // maximum and sum of the second chain's rows
+  static constexpr int kNoteOff = kStatOff + 128 * 8;  // per softmax warp: see PagedNote
+  static constexpr int kTotal = kNoteOff + 8 * 64;
   static constexpr int kDynamicBytes = kTotal + 1024;
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
 };
 
-// A CTA's way through its share of the numbered key tiles.
+// A CTA's way through its share of the line.
 struct PagedWalk {
-  int n_items, per_head;        // items; key tiles of all items for one key/value head
-  long long g, g_end;           // numbered tiles left: [g, g_end)
-  int hk, i, rem;               // where g lies: head, item, tile among per_head
+  int n_items, per_head;        // items; length of all items of one key/value head
+  long long from, to;           // the share, counted from the start of head hk
+  int hk, i;                    // next item
 };
 
 // One stretch of it: key tiles [ja, jb) of one item and head.
@@ -63,22 +72,57 @@ struct PagedSeg {
   int hk, row0, n_tok, pos0, req;
   int ja, jb, tiles;
   int seen;                     // keys the item's last token sees
-  int n_t[2];                   // key tiles of this stretch that each query tile works on
+  int n_t[2];                   // key tiles of this stretch that each warpgroup works on
   bool whole;                   // all key tiles of the item
+  bool dual;                    // one query tile in two chains: warpgroup t takes the tiles ja + t, ja + t + 2, ...
 };
 
-__device__ __forceinline__ int paged_ctas(long long total, int grid) {
-  return static_cast<int>(total < grid ? total : grid);
-}
-__device__ __forceinline__ long long paged_border(long long total, int ctas, int c) { return total * c / ctas; }
+// What a softmax warp needs between two stretches and at the end of one, but not in its loop over the key tiles, where the
+// 128 scores of a row leave no registers for it: it stands in shared memory meanwhile. (Left to the compiler, some of the loop's
+// own values were spilled: 4096 new tokens over 28k keys took 5.1 ms instead of 3.56 ms.)
+struct PagedNote {
+  PagedWalk w;
+  int row0, hk;
+  int slot;        // partial rows to write (2 * CTA or one more), or -1: the rows are complete
+  int dual, other; // dual, and whether the second chain has an accumulator
+};
 
-// Item with the largest prefix not above `rem`.
+// First key tile of an item (length `cost` per tile) that begins at or behind `at`, counted from the item's start.
+// (cost is 1 or 2; lengths of one head fit 32 bits)
+__device__ __forceinline__ int paged_tile_at(long long at, int cost) {
+  return at <= 0 ? 0 : static_cast<int>((at + cost - 1) >> (cost - 1));
+}
+
+// How the line is shared: every CTA gets `share` of it, the first `extra` ones 1 more. (Borders are then products: a quotient
+// per border, 64 bits wide, was what the combine kernel spent most of its time on.)
+struct PagedLine {
+  int ctas, extra;
+  long long share;
+  __device__ __forceinline__ PagedLine(long long total, int grid) {
+    ctas = static_cast<int>(total < grid ? total : grid);
+    share = 0;
+    if (ctas > 0) share = total <= 0x7fffffff ? static_cast<int>(total) / ctas : total / ctas;
+    extra = static_cast<int>(total - share * ctas);
+  }
+  __device__ __forceinline__ long long border(int c) const { return share * c + min(c, extra); }
+};
+// Quotient of a position on the line and the length of one head.
+__device__ __forceinline__ int paged_head(long long g, int per_head) {
+  return g <= 0x7fffffff ? static_cast<int>(g) / per_head : static_cast<int>(g / per_head);
+}
+
+// Item with the largest prefix not above `rem`. The whole warp looks at 32 items at a time: two rounds of loads for up to 1024
+// items.
 __device__ __forceinline__ int paged_find(const int* work, int n_items, int rem) {
   const int* prefix = work + kWorkHeader + 4;
-  int lo = 0, hi = n_items;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(prefix + static_cast<long long>(mid) * kWorkItem) <= rem) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = n_items;       // the item lies in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) >> 5;
+    const bool in = lane * step < n && __ldg(prefix + static_cast<long long>(lo + lane * step) * kWorkItem) <= rem;
+    const int at = max(0, __popc(__ballot_sync(0xffffffffu, in)) - 1) * step;
+    lo += at;
+    n = min(step, n - at);
   }
   return lo;
 }
@@ -87,44 +131,57 @@ __device__ __forceinline__ void paged_start(const PagedAttnDev& p, PagedWalk& w)
   w.n_items = __ldg(p.work);
   w.per_head = __ldg(p.work + 1);
   const long long total = static_cast<long long>(w.per_head) * p.Hkv;
-  const int ctas = paged_ctas(total, gridDim.x), c = blockIdx.x;
-  w.g = w.g_end = 0;
-  if (c >= ctas) return;
-  w.g = paged_border(total, ctas, c);
-  w.g_end = paged_border(total, ctas, c + 1);
-  w.hk = static_cast<int>(w.g / w.per_head);
-  w.rem = static_cast<int>(w.g - static_cast<long long>(w.hk) * w.per_head);
-  w.i = paged_find(p.work, w.n_items, w.rem);
+  const PagedLine line(total, gridDim.x);
+  const int c = blockIdx.x;
+  w.from = w.to = 0;
+  w.i = w.hk = 0;
+  if (c >= line.ctas) return;
+  const long long g = line.border(c), g_end = line.border(c + 1);
+  w.hk = paged_head(g, w.per_head);
+  const long long start = static_cast<long long>(w.hk) * w.per_head;
+  w.from = g - start;
+  w.to = g_end - start;
+  w.i = paged_find(p.work, w.n_items, static_cast<int>(w.from));
 }
 
 __device__ __forceinline__ bool paged_next(const PagedAttnDev& p, PagedWalk& w, PagedSeg& s) {
-  if (w.g >= w.g_end) return false;
-  const int4* item = reinterpret_cast<const int4*>(p.work + kWorkHeader) + 2 * static_cast<long long>(w.i);
-  const int4 a = __ldg(item), b = __ldg(item + 1);
+  int4 a, b;
+  do {
+    if (w.i == w.n_items) {
+      w.i = 0;
+      ++w.hk;
+      w.from -= w.per_head;
+      w.to -= w.per_head;
+    }
+    if (w.to <= 0) return false;
+    const int4* item = reinterpret_cast<const int4*>(p.work + kWorkHeader) + 2 * static_cast<long long>(w.i);
+    a = __ldg(item);
+    b = __ldg(item + 1);
+    if (b.x >= w.to) return false;
+    ++w.i;
+    s.ja = paged_tile_at(w.from - b.x, b.z);
+    s.jb = static_cast<int>(min(static_cast<long long>(b.y), (w.to - b.x + b.z - 1) >> (b.z - 1)));
+  } while (s.ja >= s.jb);
   s.hk = w.hk;
   s.row0 = a.x;
   s.n_tok = a.y;
   s.pos0 = a.z;
   s.req = a.w;
   s.tiles = b.y;
-  s.ja = w.rem - b.x;
-  s.jb = static_cast<int>(min(static_cast<long long>(s.tiles), s.ja + (w.g_end - w.g)));
   s.seen = min(s.pos0 + s.n_tok, p.table_width << p.page_shift);
   s.whole = s.ja == 0 && s.jb == s.tiles;
-  const int n0 = min(s.n_tok, p.tile_tokens);
+  s.dual = s.n_tok <= p.tile_tokens;
+  if (s.dual) {
+    s.n_t[0] = (s.jb - s.ja + 1) >> 1;
+    s.n_t[1] = (s.jb - s.ja) >> 1;
+    return true;
+  }
+  const int n0 = p.tile_tokens;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int last = t == 0 ? n0 : s.n_tok;      // tokens up to the end of this query tile
-    const int end = t == 0 || s.n_tok > n0 ? min(s.tiles, (s.pos0 + last + 127) >> 7) : 0;
+    const int end = min(s.tiles, (s.pos0 + last + 127) >> 7);
     s.n_t[t] = max(0, min(end, s.jb) - s.ja);
-  }
-  const int n = s.jb - s.ja;
-  w.g += n;
-  w.rem += n;
-  if (s.jb == s.tiles && ++w.i == w.n_items) {
-    w.i = 0;
-    w.rem = 0;
-    ++w.hk;
   }
   return true;
 }
@@ -156,6 +213,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   constexpr int kBlks = D / 64;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (the combine kernel may be launched from here on; it waits for this kernel's end itself)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid == 0) {
     *abort_flag = 0;
@@ -242,7 +301,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       for (int t = 0; t < 2; ++t) {
         ok = ok && mbar_wait_warp(bar_q_free(t), (seg_idx & 1u) ^ 1u, abort_flag);
         if (!ok) break;
-        if (lane == 0) {
+        if (lane == 0 && t == 1 && s.dual) {
+          mbar_arrive(bar_q_full(t));          // both chains read the first tile
+        } else if (lane == 0) {
           mbar_arrive_expect_tx(bar_q_full(t), q_bytes);
 #pragma unroll
           for (int blk = 0; blk < kBlks; ++blk)
@@ -258,22 +319,27 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (issues && key < s.seen) id = __ldg(table + (key >> p.page_shift));
         return static_cast<unsigned>(id) < static_cast<unsigned>(p.num_pages) ? id : p.num_pages;
       };
-      int next_page = page_of(s.ja);
-      for (int j = s.ja; j < s.jb && ok; ++j) {
-        const int page = next_page;
-        if (j + 1 < s.jb) next_page = page_of(j + 1);
-        const int row = (j * 128 + my_piece * piece_rows) & page_mask;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++kv_count) {
-          const int slot = kv_count % L::kStages;
-          ok = mbar_wait_warp(bar_kv_empty(slot), ((kv_count / L::kStages) & 1u) ^ 1u, abort_flag);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(bar_kv_full(slot), L::kKVTileBytes);
-          __syncwarp();
-          if (issues)
-            tma_load_5d(sKV + slot * L::kKVTileBytes + box_dst, kv ? &tmV : &tmK, bar_kv_full(slot), 0, row, my_blk, s.hk,
-                        page);
-        }
+      auto load = [&](const CUtensorMap* tm, int j, int page) {
+        const int slot = kv_count % L::kStages;
+        ok = ok && mbar_wait_warp(bar_kv_empty(slot), ((kv_count / L::kStages) & 1u) ^ 1u, abort_flag);
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_expect_tx(bar_kv_full(slot), L::kKVTileBytes);
+        __syncwarp();
+        if (issues)
+          tma_load_5d(sKV + slot * L::kKVTileBytes + box_dst, tm, bar_kv_full(slot), 0,
+                      (j * 128 + my_piece * piece_rows) & page_mask, my_blk, s.hk, page);
+        ++kv_count;
+      };
+      // in the order in which the MMA warp uses them (see there); pages are looked up two tiles ahead
+      const int n = s.jb - s.ja, ahead = s.dual ? 2 : 1;
+      int before2 = 0, before1 = 0, next = page_of(s.ja), after = n > 1 ? page_of(s.ja + 1) : 0;
+      for (int j = -ahead; j < n && ok; ++j) {
+        if (j >= 0) load(&tmV, s.ja + j, s.dual ? before2 : before1);
+        if (j + ahead < n) load(&tmK, s.ja + j + ahead, next);
+        before2 = before1;
+        before1 = next;
+        next = after;
+        if (j + ahead + 2 < n) after = page_of(s.ja + j + ahead + 2);
       }
     }
     if (!ok && lane == 0) atomicOr(p.status, 1);
@@ -285,8 +351,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const uint64_t dQ0 = make_sdesc(sQ, 16, 1024);
     const uint64_t dKV_k0 = make_sdesc(sKV, 16, 1024);               // K tile, K-major
     const uint64_t dKV_mn0 = make_sdesc(sKV, L::kBlock, 1024);       // V tile, MN-major
-    auto issue_s = [&](int t, int slot) {
-      const uint64_t a0 = sdesc_advance(dQ0, t * L::kQTileBytes);
+    auto issue_s = [&](int t, int slot, int q_tile) {
+      const uint64_t a0 = sdesc_advance(dQ0, q_tile * L::kQTileBytes);
       const uint64_t b0 = sdesc_advance(dKV_k0, slot * L::kKVTileBytes);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -313,68 +379,64 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         ok = ok && mbar_wait_warp(bar_q_full(t), seg_idx & 1u, abort_flag);
+        if (ok && (s.n_t[t] == 0 || (s.dual && t == 1))) mma_commit_e(bar_q_free(t));
         if (ok && s.n_t[t] == 0) {       // a query tile without work keeps the hand-shakes in step
-          mma_commit_e(bar_q_free(t));
           ok = mbar_wait_warp(bar_o_free(t), (seg_idx & 1u) ^ 1u, abort_flag);
           if (ok) mma_commit_e(bar_o_full(t));
         }
       }
       if (!ok) break;
-      {
-        const int slot = kv_count % L::kStages;
-        ok = mbar_wait_warp(bar_kv_full(slot), (kv_count / L::kStages) & 1u, abort_flag);
+      // Step j: O_t += P_t V_j, then S_t = Q K of the key tile `ahead` further on, for every warpgroup t whose turn it is. Two
+      // query tiles take every key tile each and look one tile ahead: while the softmax of one works, the MMAs of the other
+      // run. One query tile in two chains: chain t takes the key tiles of its parity and looks two ahead.
+      const int ahead = s.dual ? 2 : 1;
+      for (int j = -ahead; j < n && ok; ++j) {
+        const int jk = j + ahead;
+        int slot_v = 0, slot_k = 0;
+        if (j >= 0) {
+          slot_v = kv_count % L::kStages;
+          ok = mbar_wait_warp(bar_kv_full(slot_v), (kv_count / L::kStages) & 1u, abort_flag);
+          ++kv_count;
+          if (ok && j == n - 1 && s.jb == s.tiles && (s.seen & 127) != 0) {
+            if (lane == 0) mbar_arrive(bar_dirty);
+            __syncwarp();
+            ok = mbar_wait_warp(bar_clean, turn & 1u, abort_flag);
+            ++turn;
+          }
+        }
+        if (ok && jk < n) {
+          slot_k = kv_count % L::kStages;
+          ok = mbar_wait_warp(bar_kv_full(slot_k), (kv_count / L::kStages) & 1u, abort_flag);
+          ++kv_count;
+        }
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (s.n_t[t] > 0) {
-            issue_s(t, slot);
-            if (s.n_t[t] == 1) mma_commit_e(bar_q_free(t));   // that was the last S of tile t
-          }
-        }
-        mma_commit_e(bar_kv_empty(slot));
-        ++kv_count;
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        const bool has_next = j + 1 < n;
-        const int slot_v = kv_count % L::kStages, slot_k = (kv_count + 1) % L::kStages;
-        ok = mbar_wait_warp(bar_kv_full(slot_v), (kv_count / L::kStages) & 1u, abort_flag);
-        if (ok && has_next) ok = mbar_wait_warp(bar_kv_full(slot_k), ((kv_count + 1) / L::kStages) & 1u, abort_flag);
-        if (ok && !has_next && s.jb == s.tiles && (s.seen & 127) != 0) {
-          if (lane == 0) mbar_arrive(bar_dirty);
-          __syncwarp();
-          ok = mbar_wait_warp(bar_clean, turn & 1u, abort_flag);
-          ++turn;
-        }
-        if (!ok) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j < s.n_t[t]) {
-            if (j == 0) {      // the epilogue of the previous stretch has read O_t out of tensor memory
-              ok = mbar_wait_warp(bar_o_free(t), (seg_idx & 1u) ^ 1u, abort_flag);
-              if (!ok) break;
-            }
+          const bool mine = !s.dual || (j & 1) == t;
+          const int last = s.dual ? n : s.n_t[t];            // key tiles this warpgroup works on end here
+          const bool pv = mine && j >= 0 && j < last;
+          if (pv) {
+            if (j < ahead) ok = mbar_wait_warp(bar_o_free(t), (seg_idx & 1u) ^ 1u, abort_flag);   // O_t has been read out
 #pragma unroll
             for (int hh = 0; hh < kPSplit; ++hh) {
-              ok = mbar_wait_warp(bar_p_full(t, hh), it_cnt[t] & 1u, abort_flag);
+              if (ok) ok = mbar_wait_warp(bar_p_full(t, hh), it_cnt[t] & 1u, abort_flag);
               if (!ok) break;
               tc_fence_after();
-              issue_o(t, slot_v, j == 0, hh);
+              issue_o(t, slot_v, j < ahead, hh);
             }
             if (!ok) break;
             ++it_cnt[t];
-            if (j + 1 < s.n_t[t]) {
-              issue_s(t, slot_k);
-              if (j + 2 == s.n_t[t]) mma_commit_e(bar_q_free(t));   // last S of tile t issued
-            } else {
-              mma_commit_e(bar_o_full(t));
-            }
           }
+          if (mine && jk < last) {
+            issue_s(t, slot_k, s.dual ? 0 : t);
+            if (s.dual ? jk == n - 1 : jk + 1 == last) mma_commit_e(bar_q_free(s.dual ? 0 : t));   // the last S of the Q tile
+          }
+          if (pv && jk >= last) mma_commit_e(bar_o_full(t));
         }
         if (!ok) break;
-        mma_commit_e(bar_kv_empty(slot_v));
-        if (has_next) mma_commit_e(bar_kv_empty(slot_k));
-        kv_count += has_next ? 2 : 1;
+        if (j >= 0) mma_commit_e(bar_kv_empty(slot_v));
+        if (jk < n) mma_commit_e(bar_kv_empty(slot_k));
       }
     }
     if (!ok && lane == 0) atomicOr(p.status, 2);
@@ -386,29 +448,64 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const uint32_t tS = tmem_base + lane_base + kColS + t * kBN;
     const uint32_t tO = tmem_base + lane_base + kColO + t * D;
     const float sc = ModTerms<kMod>::sc(p.scale_log2, p.cap2);
-    const int tok = r / p.G, head = r - tok * p.G;     // this row's token in the tile and head in the group
+    static_assert(sizeof(PagedNote) <= 64, "the notes overlap");
+    volatile PagedNote* note = reinterpret_cast<volatile PagedNote*>(smem_gen + L::kNoteOff + warp * 64);
     FwdKernelParams none;                              // softmax_tile_row reads nothing of it without score terms
     const KeepBitsDropout keep{false, make_uint4(0u, 0u, 0u, 0u)};
     uint32_t it_cnt = 0, o_cnt = 0;
     bool ok = true;
-    PagedWalk w;
-    PagedSeg s;
-    paged_start(p, w);
-    while (paged_next(p, w, s)) {
-      const int nt = s.n_t[t];
-      const int tokens = min(p.tile_tokens, max(0, s.n_tok - t * p.tile_tokens));   // of this query tile
-      const bool valid = tok < tokens;
-      const bool live = 32 * (warp & 3) < tokens * p.G;    // some row of the warp is
-      const int pos = s.pos0 + t * p.tile_tokens + tok;
-      const int row_lim = valid ? min(pos, s.seen - 1) : -1;
-      const int h = s.hk * p.G + head;
+    {
+      PagedWalk w;
+      paged_start(p, w);
+      if (lane == 0) {
+        note->w.n_items = w.n_items; note->w.per_head = w.per_head;
+        note->w.from = w.from; note->w.to = w.to;
+        note->w.hk = w.hk; note->w.i = w.i;
+      }
+      __syncwarp();
+    }
+    while (true) {
+      int nt, row_lim, tile, tile_step, pos;
+      float slope_h = 0.f;
+      bool live;
+      {
+        PagedWalk w;
+        w.n_items = note->w.n_items; w.per_head = note->w.per_head;
+        w.from = note->w.from; w.to = note->w.to;
+        w.hk = note->w.hk; w.i = note->w.i;
+        PagedSeg s;
+        if (!paged_next(p, w, s)) break;
+        const int tok = r / p.G, head = r - tok * p.G;     // this row's token in the tile and head in the group
+        const int tok0 = s.dual ? 0 : t * p.tile_tokens;   // first token of this query tile
+        const int tokens = min(p.tile_tokens, max(0, s.n_tok - tok0));
+        const bool valid = tok < tokens;
+        live = 32 * (warp & 3) < tokens * p.G;             // some row of the warp is
+        nt = s.n_t[t];
+        tile = s.dual ? s.ja + t : s.ja;
+        tile_step = s.dual ? 2 : 1;
+        pos = s.pos0 + tok0 + tok;
+        row_lim = valid ? min(pos, s.seen - 1) : -1;
+        if (has_slope(kMod) && valid) slope_h = __ldg(p.slopes + s.hk * p.G + head);
+        __syncwarp();
+        if (lane == 0) {
+          note->w.from = w.from; note->w.to = w.to;
+          note->w.hk = w.hk; note->w.i = w.i;
+          note->row0 = s.row0 + tok0;
+          note->hk = s.hk;
+          // the first stretch of a CTA that begins inside an item, the last one that ends inside one
+          note->slot = s.whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (s.ja > 0 ? 0 : 1);
+          note->dual = s.dual;
+          note->other = s.dual && s.n_t[1] > 0;
+        }
+        __syncwarp();
+      }
       float m = -INFINITY, l = 0.f;
-      const ModTerms<kMod> terms(p.scale_log2, p.arg2, p.cap2, has_slope(kMod) && valid ? __ldg(p.slopes + h) : 0.f, pos);
-      for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
+      const ModTerms<kMod> terms(p.scale_log2, p.arg2, p.cap2, slope_h, pos);
+      for (int j = 0; j < nt && ok; ++j, ++it_cnt, tile += tile_step) {
         ok = mbar_wait(bar_s_full(t), it_cnt & 1u, abort_flag);
         if (!ok) break;
         if (live) {
-          softmax_tile_row<D, kBf16, false, true>(tS, tO, s.ja + j, j > 0, none, row_lim, sc, false, m, l, [] {},
+          softmax_tile_row<D, kBf16, false, true>(tS, tO, tile, j > 0, none, row_lim, sc, false, m, l, [] {},
                                                   [&](int hh) { mbar_arrive(bar_p_full(t, hh)); }, terms, keep, 0);
         } else {
           // rows nobody asked for: whatever stands in their P only reaches rows of O that are not read
@@ -419,13 +516,31 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (ok) ok = mbar_wait(bar_o_full(t), o_cnt & 1u, abort_flag);   // once per stretch, work or not
       ++o_cnt;
       tc_fence_after();
+      float mine = 1.f, other = 0.f;       // factors of the two chains' accumulators
+      const bool dual = note->dual != 0;
+      if (dual) {
+        // (a thread whose wait gave up meets the others here all the same)
+        float2* stat = reinterpret_cast<float2*>(smem_gen + L::kStatOff);
+        if (t == 1) stat[r] = make_float2(m, l);
+        named_bar_sync(1, 256);
+        if (t == 1) continue;              // the first warpgroup writes the rows and hands both accumulators back
+        const float2 o = stat[r];
+        const float top = fmaxf(m, o.x);
+        if (top > -INFINITY) {
+          mine = ex2_approx((m - top) * sc);
+          other = ex2_approx((o.x - top) * sc);
+        }
+        m = top;
+        l = l * mine + o.y * other;
+      }
       const float inv = l > 0.f ? 1.f / l : 0.f;
       const float lse2 = l > 0.f ? m * sc + lg2_approx(l) : -INFINITY;
-      const long long token = s.row0 + t * p.tile_tokens + tok;
-      // partial results: the first stretch of a CTA that begins inside an item, the last one that ends inside one
-      const long long prow = (2LL * blockIdx.x + (s.ja > 0 ? 0 : 1)) * 256 + t * kBM + r;
+      const int tok = r / p.G, h = note->hk * p.G + (r - tok * p.G), slot = note->slot;
+      const bool valid = row_lim >= 0, whole = slot < 0, join = note->other != 0;
+      const long long token = note->row0 + tok;
+      const long long prow = static_cast<long long>(slot) * 256 + t * kBM + r;
       if (ok && valid) {
-        if (s.whole) {
+        if (whole) {
           if (p.lse) p.lse[token * p.Hq + h] = lse2 * kLn2;
         } else {
           p.part_lse[prow] = lse2;
@@ -441,12 +556,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = 0u;
         }
+        if (join && live) {
+          uint32_t o1[32];
+          tmem_ld32(tO + D + c * 32, o1);
+          tc_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            o[k] = __float_as_uint(__uint_as_float(o[k]) * mine + __uint_as_float(o1[k]) * other);
+        }
         if (c == D / 32 - 1) {
           tc_fence_before();
           mbar_arrive(bar_o_free(t));
+          if (dual) mbar_arrive(bar_o_free(1));
         }
         if (ok && valid) {
-          if (s.whole) {
+          if (whole) {
             const int col = (c & 1) * 32;                       // column inside the 64-column block
             uint4* dst = reinterpret_cast<uint4*>(p.out + token * p.out_st + h * p.out_sh + (c >> 1) * p.blk + col);
 #pragma unroll
@@ -479,25 +603,33 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 // Joins the partial rows of an item cut by CTA borders: with the parts' log2 sums L_c,
 //   out = sum_c 2^(L_c - L) o_c,   L = log2 sum_c 2^L_c,
 // in the order of the keys. Block (c, y) looks at the border between CTA c and c + 1 and works iff that border is the first
-// inside its item; one warp per row, rows dealt over the y blocks. Reads each partial row once.
+// inside its item; one warp per row, rows dealt over the y blocks. Reads each partial row once. It is launched while the main
+// kernel still runs (programmatic dependent launch) and waits for its results only after it has found its item.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256)
 paged_combine_kernel(const PagedAttnDev p, int main_grid) {
   const int n_items = __ldg(p.work), per_head = __ldg(p.work + 1);
   const long long total = static_cast<long long>(per_head) * p.Hkv;
-  const int ctas = paged_ctas(total, main_grid);
-  const int c = blockIdx.x + 1;
-  if (c >= ctas) return;
-  const long long g = paged_border(total, ctas, c);
-  const int hk = static_cast<int>(g / per_head);
+  const PagedLine line(total, main_grid);
+  const int c = blockIdx.x + 1, ctas = line.ctas;
+  if (c >= ctas) {
+    // (every block waits, so that this kernel never ends before the main one)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const long long g = line.border(c);
+  const int hk = paged_head(g, per_head);
   const int rem = static_cast<int>(g - static_cast<long long>(hk) * per_head);
   const int i = paged_find(p.work, n_items, rem);
   const int4* item = reinterpret_cast<const int4*>(p.work + kWorkHeader) + 2 * static_cast<long long>(i);
   const int4 a = __ldg(item), b = __ldg(item + 1);
-  const long long begin = static_cast<long long>(hk) * per_head + b.x, end = begin + b.y;
-  if (g == begin || paged_border(total, ctas, c - 1) > begin) return;
+  const long long begin = static_cast<long long>(hk) * per_head + b.x;
+  auto tile_at = [&](int cc) { return paged_tile_at(line.border(cc) - begin, b.z); };   // border of CTA cc
+  const bool first_inside = tile_at(c) > 0 && tile_at(c) < b.y && tile_at(c - 1) <= 0;
   int last = c;      // last CTA with a part of the item
-  while (last + 1 < ctas && paged_border(total, ctas, last + 1) < end) ++last;
+  while (first_inside && last + 1 < ctas && tile_at(last + 1) < b.y) ++last;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!first_inside) return;
 
   const int lane = threadIdx.x & 31;
   const int rows = a.y * p.G;
@@ -507,8 +639,12 @@ paged_combine_kernel(const PagedAttnDev p, int main_grid) {
     const int t = tok >= p.tile_tokens ? 1 : 0;
     const int r = t * kBM + x - t * p.tile_tokens * p.G;     // row inside the parts
     auto row_of = [&](int cc) { return (cc == c - 1 ? 2LL * cc + 1 : 2LL * cc) * 256 + r; };
+    // log2 sum of CTA cc's part; -inf: it has none (its share of the line holds the start of no tile)
+    auto part = [&](int cc) {
+      return cc < c || tile_at(cc) < min(b.y, tile_at(cc + 1)) ? __ldcg(p.part_lse + row_of(cc)) : -INFINITY;
+    };
     float m = -INFINITY;
-    for (int cc = c - 1 + lane; cc <= last; cc += 32) m = fmaxf(m, __ldg(p.part_lse + row_of(cc)));
+    for (int cc = c - 1 + lane; cc <= last; cc += 32) m = fmaxf(m, part(cc));
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     float acc[kVec], sum = 0.f;
@@ -517,17 +653,19 @@ paged_combine_kernel(const PagedAttnDev p, int main_grid) {
     if (m > -INFINITY) {
 #pragma unroll 4
       for (int cc = c - 1; cc <= last; ++cc) {
-        const float wgt = ex2_approx(__ldg(p.part_lse + row_of(cc)) - m);
+        const float lse = part(cc);
+        if (lse == -INFINITY) continue;
+        const float wgt = ex2_approx(lse - m);
         const float* src = p.part_o + row_of(cc) * D + lane * kVec;
         sum += wgt;
         if constexpr (kVec == 4) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(src));
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
           acc[0] = fmaf(wgt, v.x, acc[0]);
           acc[1] = fmaf(wgt, v.y, acc[1]);
           acc[2] = fmaf(wgt, v.z, acc[2]);
           acc[3] = fmaf(wgt, v.w, acc[3]);
         } else {
-          const float2 v = __ldg(reinterpret_cast<const float2*>(src));
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
           acc[0] = fmaf(wgt, v.x, acc[0]);
           acc[1] = fmaf(wgt, v.y, acc[1]);
         }
@@ -556,8 +694,17 @@ static cudaError_t launch_paged_one(const PagedAttnLaunch& a, cudaStream_t strea
   kern<<<grid, kPagedThreads, L::kDynamicBytes, stream>>>(a.tmQ, a.tmK, a.tmV, a.p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (grid > 1) paged_combine_kernel<D, kBf16><<<dim3(grid - 1, 4), 256, 0, stream>>>(a.p, grid);
-  return cudaGetLastError();
+  if (grid < 2) return cudaSuccess;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid - 1, 4);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, kBf16>, a.p, grid);
 }
 
 template <int D>

@@ -6,7 +6,7 @@
 //   fresh_b = sum over the requests before b of need - have: its pages in the list of free ones start there
 //   token i of it: position c_b + i, slot = page(position >> s) * 2^s + position mod 2^s
 // and the work list of the attention: items of `item_tokens` query tokens with the number of 128-key tiles that each
-// of them sees and the sum of those before it.
+// of them sees, what a tile costs (2 if the tokens need both query tiles, else 1) and the cost of the items before it.
 //
 // One launch. Every block scans the requests by itself in shared memory (a few thousand numbers: cheaper than a second
 // launch that waits for the first), then block 0 writes the work list while the others place tokens, one per thread.
@@ -146,6 +146,7 @@ paged_plan_kernel(const PagedPlanDev p) {
     const int i = base + tid;
     int4 a = make_int4(0, 0, 0, 0);
     long long tiles = 0;
+    int cost = 1;
     if (i < n_items) {
       const int r = last_not_above(first_item, p.B, i);
       const int t0 = (i - first_item[r]) * p.item_tokens;
@@ -153,12 +154,13 @@ paged_plan_kernel(const PagedPlanDev p) {
       const long long pos0 = context(r) + t0;
       a = make_int4(cu[r] + t0, n, static_cast<int>(min(pos0, static_cast<long long>(INT_MAX / 2))), r);
       tiles = max(1LL, (min(pos0 + n, capacity) + 127) >> 7);
+      cost = 2 * n > p.item_tokens ? 2 : 1;
     }
     long long all;
-    const long long before = carry + block_exclusive(tiles, warp_tot, all);
+    const long long before = carry + block_exclusive(tiles * cost, warp_tot, all);
     if (i < n_items) {
       items[2 * i] = a;
-      items[2 * i + 1] = make_int4(static_cast<int>(before), static_cast<int>(tiles), 0, 0);
+      items[2 * i + 1] = make_int4(static_cast<int>(before), static_cast<int>(tiles), cost, 0);
     }
     carry += all;
   }

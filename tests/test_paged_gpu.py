@@ -93,8 +93,9 @@ def test_work_list_covers_every_token_once(heads_q, heads_kv):
         for t in range(0, n, per):
             m = min(per, n - t)
             tiles = -(-(c + t + m) // 128)
-            want.append([sum(new[:b]) + t, m, c + t, b, before, tiles, 0, 0])
-            before += tiles
+            cost = 2 if 2 * m > per else 1      # a tile of an item that fills both query tiles counts twice
+            want.append([sum(new[:b]) + t, m, c + t, b, before, tiles, cost, 0])
+            before += cost * tiles
     work = plan.work.tolist()
     assert work[:2] == [len(want), before]
     assert work[16:16 + 8 * len(want)] == [x for w in want for x in w]
