@@ -88,6 +88,7 @@ typedef struct {
   size_t work_bytes;            /* at least fa2_paged_work_bytes                                   */
 } fa2_paged_plan_params;
 
+/* Depends, like the plan itself, on the current device's number of SMs. */
 size_t fa2_paged_work_bytes(int32_t requests, int32_t num_tokens, int32_t heads_q, int32_t heads_kv);
 int fa2_paged_plan(const fa2_paged_plan_params* params, void* cuda_stream);
 

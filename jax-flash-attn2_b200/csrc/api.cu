@@ -602,8 +602,8 @@ int encode_map(CUtensorMap* tm, const void* ptr, bool bf16, const cuuint64_t (&d
 
 size_t fa2_paged_work_bytes(int32_t requests, int32_t num_tokens, int32_t heads_q, int32_t heads_kv) {
   if (requests <= 0 || num_tokens < 0 || check_groups(heads_q, heads_kv)) return 0;
-  return (kWorkHeader + kWorkItem * static_cast<size_t>(max_items(requests, num_tokens, item_tokens_of(heads_q, heads_kv)))) *
-         sizeof(int32_t);
+  return (work_items_at(sm_count()) +
+          kWorkItem * static_cast<size_t>(max_items(requests, num_tokens, item_tokens_of(heads_q, heads_kv)))) * sizeof(int32_t);
 }
 
 int fa2_paged_plan(const fa2_paged_plan_params* a, void* cuda_stream) {
@@ -631,10 +631,10 @@ int fa2_paged_plan(const fa2_paged_plan_params* a, void* cuda_stream) {
     return fail(FA2_ERR_INVALID_ARG, "slot_map must be 8-byte and work 16-byte aligned");
   const int item_tokens = item_tokens_of(a->heads_q, a->heads_kv);
   const int64_t items = max_items(a->requests, a->num_tokens, item_tokens);
-  if (a->work_bytes < (kWorkHeader + kWorkItem * static_cast<size_t>(items)) * sizeof(int32_t))
+  if (a->work_bytes < (work_items_at(sm_count()) + kWorkItem * static_cast<size_t>(items)) * sizeof(int32_t))
     return fail(FA2_ERR_WORKSPACE, "work must hold fa2_paged_work_bytes bytes");
   const int64_t tiles = ((static_cast<int64_t>(a->table_width) << shift) + 127) / 128;
-  if (2 * items * tiles > INT_MAX)
+  if (2 * items * (tiles + 2) > INT_MAX)
     return fail(FA2_ERR_UNSUPPORTED, "problem too large: %lld items of up to %lld key tiles must stay below 2^30",
                 static_cast<long long>(items), static_cast<long long>(tiles));
   PagedPlanDev d;
@@ -650,6 +650,9 @@ int fa2_paged_plan(const fa2_paged_plan_params* a, void* cuda_stream) {
   d.page_shift = shift;
   d.num_tokens = a->num_tokens;
   d.item_tokens = item_tokens;
+  d.heads_kv = a->heads_kv;
+  d.sms = sm_count();
+  d.items_at = work_items_at(d.sms);
   d.cu_seqlens = a->cu_seqlens;
   d.seqlens_k = a->seqlens_k;
   d.slot_map = reinterpret_cast<long long*>(a->slot_map);
@@ -778,6 +781,7 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
   d.T = a->tokens; d.Hq = a->heads_q; d.Hkv = a->heads_kv; d.G = group;
   d.tile_tokens = tile_tokens;
   d.work = a->work;
+  d.items_at = work_items_at(sm_count());
   d.block_table = a->block_table;
   d.table_stride = a->table_stride;
   d.table_width = a->table_width;

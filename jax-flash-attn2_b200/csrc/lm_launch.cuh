@@ -9,11 +9,15 @@ namespace fa2 {
 
 cudaError_t launch_document_layout(const int* ids, long long stride_b, int B, int S, int* layout, cudaStream_t stream);
 
-// Work list of the paged attention (int32): a header of kWorkHeader words (0: items, 1: cost of all items together),
-// then kWorkItem words per item: first row of the packed tensors, tokens, position of the first token, request, cost of
-// the items before it, key tiles of its own, cost of a key tile (1 or 2), 0.
+// Work list of the paged attention (int32):
+//   header     kWorkHeader words: 0: items, 1: CTAs that get a share
+//   starts     where every CTA starts and, behind the last one, the end: 4 words (key/value head, item, key tile, 0) for each
+//              of the device's SMs and one more
+//   items      kWorkItem words each: first row of the packed tensors, tokens, position of the first token, request, cost of
+//              the items before it, key tiles of its own, cost of a key tile (1 or 2), 0
 constexpr int kWorkHeader = 16;
 constexpr int kWorkItem = 8;
+inline int work_items_at(int sms) { return kWorkHeader + (4 * (sms + 1) + 7) / 8 * 8; }   // word of the first item
 
 struct PagedPlanDev {
   const int *context_lens, *new_lens;
@@ -27,6 +31,7 @@ struct PagedPlanDev {
   int page_shift;
   int num_tokens;
   int item_tokens;           // query tokens per item of the work list
+  int heads_kv, sms, items_at;
   int *cu_seqlens, *seqlens_k;
   long long* slot_map;
   int *positions, *pages_taken, *work;
@@ -49,6 +54,7 @@ struct PagedAttnDev {
   int T, Hq, Hkv, G;
   int tile_tokens;           // tokens of a 128-row tile: floor(128 / G)
   const int* work;
+  int items_at;
   const int* block_table;
   long long table_stride;
   int table_width, page_shift, num_pages;

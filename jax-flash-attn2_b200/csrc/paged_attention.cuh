@@ -7,10 +7,9 @@
 // read once per group: a 128-row tile holds floor(128 / G) tokens, an item (two tiles over one stream of keys, as in
 // fwd_kernel.cuh) twice as many.
 //
-// Split. The key tiles of all items of all key/value heads stand on one line, W long in all, on which a tile of a two-tile item
-// takes 2 and one of a smaller item 1 (what they cost: see "Few rows"), and CTA c works on the tiles that begin in
-// [c W / n, (c + 1) W / n): every SM gets the same share whatever the lengths of the requests are. A CTA that has all key
-// tiles of an item writes its rows; items cut by a border leave normalised partial rows and their log-sum-exp in
+// Split. The plan deals the key tiles of all items of all key/value heads to the CTAs in one line, in equal shares whatever
+// the lengths of the requests are (paged_plan.cu), and notes where each CTA starts. A CTA that has all key tiles of an item
+// writes its rows; items cut by a border leave normalised partial rows and their log-sum-exp in
 // float32 (at most two per CTA), which paged_combine_kernel joins in the order of the keys: the result does not depend on
 // which CTA was faster.
 //
@@ -60,11 +59,11 @@ struct PagedSmem {
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
 };
 
-// A CTA's way through its share of the line.
+// A CTA's way from its start to the next CTA's.
 struct PagedWalk {
-  int n_items, per_head;        // items; length of all items of one key/value head
-  long long from, to;           // the share, counted from the start of head hk
-  int hk, i;                    // next item
+  int n_items;
+  int hk, i, tile;
+  int end_hk, end_i, end_tile;
 };
 
 // One stretch of it: key tiles [ja, jb) of one item and head.
@@ -87,89 +86,43 @@ struct PagedNote {
   int dual, other; // dual, and whether the second chain has an accumulator
 };
 
-// First key tile of an item (length `cost` per tile) that begins at or behind `at`, counted from the item's start.
-// (cost is 1 or 2; lengths of one head fit 32 bits)
-__device__ __forceinline__ int paged_tile_at(long long at, int cost) {
-  return at <= 0 ? 0 : static_cast<int>((at + cost - 1) >> (cost - 1));
-}
-
-// How the line is shared: every CTA gets `share` of it, the first `extra` ones 1 more. (Borders are then products: a quotient
-// per border, 64 bits wide, was what the combine kernel spent most of its time on.)
-struct PagedLine {
-  int ctas, extra;
-  long long share;
-  __device__ __forceinline__ PagedLine(long long total, int grid) {
-    ctas = static_cast<int>(total < grid ? total : grid);
-    share = 0;
-    if (ctas > 0) share = total <= 0x7fffffff ? static_cast<int>(total) / ctas : total / ctas;
-    extra = static_cast<int>(total - share * ctas);
-  }
-  __device__ __forceinline__ long long border(int c) const { return share * c + min(c, extra); }
-};
-// Quotient of a position on the line and the length of one head.
-__device__ __forceinline__ int paged_head(long long g, int per_head) {
-  return g <= 0x7fffffff ? static_cast<int>(g) / per_head : static_cast<int>(g / per_head);
-}
-
-// Item with the largest prefix not above `rem`. The whole warp looks at 32 items at a time: two rounds of loads for up to 1024
-// items.
-__device__ __forceinline__ int paged_find(const int* work, int n_items, int rem) {
-  const int* prefix = work + kWorkHeader + 4;
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = n_items;       // the item lies in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + 31) >> 5;
-    const bool in = lane * step < n && __ldg(prefix + static_cast<long long>(lo + lane * step) * kWorkItem) <= rem;
-    const int at = max(0, __popc(__ballot_sync(0xffffffffu, in)) - 1) * step;
-    lo += at;
-    n = min(step, n - at);
-  }
-  return lo;
+__device__ __forceinline__ int4 paged_start_of(const int* work, int c) {
+  return __ldg(reinterpret_cast<const int4*>(work + kWorkHeader) + c);
 }
 
 __device__ __forceinline__ void paged_start(const PagedAttnDev& p, PagedWalk& w) {
   w.n_items = __ldg(p.work);
-  w.per_head = __ldg(p.work + 1);
-  const long long total = static_cast<long long>(w.per_head) * p.Hkv;
-  const PagedLine line(total, gridDim.x);
-  const int c = blockIdx.x;
-  w.from = w.to = 0;
-  w.i = w.hk = 0;
-  if (c >= line.ctas) return;
-  const long long g = line.border(c), g_end = line.border(c + 1);
-  w.hk = paged_head(g, w.per_head);
-  const long long start = static_cast<long long>(w.hk) * w.per_head;
-  w.from = g - start;
-  w.to = g_end - start;
-  w.i = paged_find(p.work, w.n_items, static_cast<int>(w.from));
+  const int ctas = __ldg(p.work + 1), c = blockIdx.x;
+  w.hk = w.i = w.tile = w.end_hk = w.end_i = w.end_tile = 0;
+  if (c >= ctas) return;
+  const int4 from = paged_start_of(p.work, c), to = paged_start_of(p.work, c + 1);
+  w.hk = from.x; w.i = from.y; w.tile = from.z;
+  w.end_hk = to.x; w.end_i = to.y; w.end_tile = to.z;
 }
 
 __device__ __forceinline__ bool paged_next(const PagedAttnDev& p, PagedWalk& w, PagedSeg& s) {
-  int4 a, b;
-  do {
-    if (w.i == w.n_items) {
-      w.i = 0;
-      ++w.hk;
-      w.from -= w.per_head;
-      w.to -= w.per_head;
-    }
-    if (w.to <= 0) return false;
-    const int4* item = reinterpret_cast<const int4*>(p.work + kWorkHeader) + 2 * static_cast<long long>(w.i);
-    a = __ldg(item);
-    b = __ldg(item + 1);
-    if (b.x >= w.to) return false;
-    ++w.i;
-    s.ja = paged_tile_at(w.from - b.x, b.z);
-    s.jb = static_cast<int>(min(static_cast<long long>(b.y), (w.to - b.x + b.z - 1) >> (b.z - 1)));
-  } while (s.ja >= s.jb);
+  const bool in_last = w.hk == w.end_hk && w.i == w.end_i;
+  if (in_last && w.tile >= w.end_tile) return false;
+  const int4* item = reinterpret_cast<const int4*>(p.work + p.items_at) + 2 * static_cast<long long>(w.i);
+  const int4 a = __ldg(item);
+  s.tiles = __ldg(&item[1].y);
   s.hk = w.hk;
   s.row0 = a.x;
   s.n_tok = a.y;
   s.pos0 = a.z;
   s.req = a.w;
-  s.tiles = b.y;
+  s.ja = w.tile;
+  s.jb = in_last ? w.end_tile : s.tiles;
   s.seen = min(s.pos0 + s.n_tok, p.table_width << p.page_shift);
   s.whole = s.ja == 0 && s.jb == s.tiles;
+  w.tile = s.jb;
+  if (s.jb == s.tiles) {
+    w.tile = 0;
+    if (++w.i == w.n_items) {
+      w.i = 0;
+      ++w.hk;
+    }
+  }
   s.dual = s.n_tok <= p.tile_tokens;
   if (s.dual) {
     s.n_t[0] = (s.jb - s.ja + 1) >> 1;
@@ -213,6 +166,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   constexpr int kBlks = D / 64;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 9 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  PagedWalk w;                 // (its loads are under way while the barriers are set up)
+  paged_start(p, w);
   // (the combine kernel may be launched from here on; it waits for this kernel's end itself)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -234,11 +194,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     mbar_init(bar_clean, 1);
     fence_mbar_init();
   }
-  if (warp == 9 && lane == 0) {
-    tma_prefetch_desc(&tmQ);
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
-  }
   if (warp == 0) {
     __syncwarp();
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -256,9 +211,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     // =========================== clears V rows behind the last visible key ==================
     bool ok = true;
     uint32_t kv_count = 0, turn = 0;
-    PagedWalk w;
     PagedSeg s;
-    paged_start(p, w);
     while (ok && paged_next(p, w, s)) {
       const int tail = s.seen & 127;
       kv_count += 2 * (s.jb - s.ja);
@@ -287,9 +240,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     // =========================== TMA producer ================================================
     bool ok = true;
     uint32_t kv_count = 0, seg_idx = 0;
-    PagedWalk w;
     PagedSeg s;
-    paged_start(p, w);
     const int piece_rows = min(128, 1 << p.page_shift), pieces = 128 / piece_rows;
     const int my_piece = lane % pieces, my_blk = lane / pieces;    // this lane's box of a K or V tile
     const bool issues = my_blk < kBlks;
@@ -371,9 +322,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     uint32_t kv_count = 0, seg_idx = 0;
     uint32_t turn = 0;             // V tiles cleared so far
     uint32_t it_cnt[2] = {0, 0};
-    PagedWalk w;
     PagedSeg s;
-    paged_start(p, w);
     for (; ok && paged_next(p, w, s); ++seg_idx) {
       const int n = s.jb - s.ja;
 #pragma unroll
@@ -454,25 +403,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const KeepBitsDropout keep{false, make_uint4(0u, 0u, 0u, 0u)};
     uint32_t it_cnt = 0, o_cnt = 0;
     bool ok = true;
-    {
-      PagedWalk w;
-      paged_start(p, w);
-      if (lane == 0) {
-        note->w.n_items = w.n_items; note->w.per_head = w.per_head;
-        note->w.from = w.from; note->w.to = w.to;
-        note->w.hk = w.hk; note->w.i = w.i;
-      }
-      __syncwarp();
+    if (lane == 0) {
+      note->w.n_items = w.n_items;
+      note->w.hk = w.hk; note->w.i = w.i; note->w.tile = w.tile;
+      note->w.end_hk = w.end_hk; note->w.end_i = w.end_i; note->w.end_tile = w.end_tile;
     }
+    __syncwarp();
     while (true) {
       int nt, row_lim, tile, tile_step, pos;
       float slope_h = 0.f;
       bool live;
       {
-        PagedWalk w;
-        w.n_items = note->w.n_items; w.per_head = note->w.per_head;
-        w.from = note->w.from; w.to = note->w.to;
-        w.hk = note->w.hk; w.i = note->w.i;
+        w.n_items = note->w.n_items;
+        w.hk = note->w.hk; w.i = note->w.i; w.tile = note->w.tile;
+        w.end_hk = note->w.end_hk; w.end_i = note->w.end_i; w.end_tile = note->w.end_tile;
         PagedSeg s;
         if (!paged_next(p, w, s)) break;
         const int tok = r / p.G, head = r - tok * p.G;     // this row's token in the tile and head in the group
@@ -488,8 +432,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (has_slope(kMod) && valid) slope_h = __ldg(p.slopes + s.hk * p.G + head);
         __syncwarp();
         if (lane == 0) {
-          note->w.from = w.from; note->w.to = w.to;
-          note->w.hk = w.hk; note->w.i = w.i;
+          note->w.hk = w.hk; note->w.i = w.i; note->w.tile = w.tile;
           note->row0 = s.row0 + tok0;
           note->hk = s.hk;
           // the first stretch of a CTA that begins inside an item, the last one that ends inside one
@@ -600,86 +543,128 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   }
 }
 
-// Joins the partial rows of an item cut by CTA borders: with the parts' log2 sums L_c,
-//   out = sum_c 2^(L_c - L) o_c,   L = log2 sum_c 2^L_c,
-// in the order of the keys. Block (c, y) looks at the border between CTA c and c + 1 and works iff that border is the first
-// inside its item; one warp per row, rows dealt over the y blocks. Reads each partial row once. It is launched while the main
-// kernel still runs (programmatic dependent launch) and waits for its results only after it has found its item.
-template <int D, bool kBf16>
-__global__ void __launch_bounds__(256)
-paged_combine_kernel(const PagedAttnDev p, int main_grid) {
-  const int n_items = __ldg(p.work), per_head = __ldg(p.work + 1);
-  const long long total = static_cast<long long>(per_head) * p.Hkv;
-  const PagedLine line(total, main_grid);
-  const int c = blockIdx.x + 1, ctas = line.ctas;
-  if (c >= ctas) {
-    // (every block waits, so that this kernel never ends before the main one)
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
-  const long long g = line.border(c);
-  const int hk = paged_head(g, per_head);
-  const int rem = static_cast<int>(g - static_cast<long long>(hk) * per_head);
-  const int i = paged_find(p.work, n_items, rem);
-  const int4* item = reinterpret_cast<const int4*>(p.work + kWorkHeader) + 2 * static_cast<long long>(i);
-  const int4 a = __ldg(item), b = __ldg(item + 1);
-  const long long begin = static_cast<long long>(hk) * per_head + b.x;
-  auto tile_at = [&](int cc) { return paged_tile_at(line.border(cc) - begin, b.z); };   // border of CTA cc
-  const bool first_inside = tile_at(c) > 0 && tile_at(c) < b.y && tile_at(c - 1) <= 0;
-  int last = c;      // last CTA with a part of the item
-  while (first_inside && last + 1 < ctas && tile_at(last + 1) < b.y) ++last;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!first_inside) return;
-
-  const int lane = threadIdx.x & 31;
-  const int rows = a.y * p.G;
+// kRows rows of an item at a time, x0, x0 + stride, ...; the parts of CTAs c - 1 .. last that `parts` says are there (bit i:
+// CTA base + i, 32 at a time), kParts of them with their loads under way at once: a part's row comes from L2, and one after
+// the other they would cost its latency each.
+template <int D, bool kBf16, int kRows, int kParts>
+__device__ __forceinline__ void paged_join_rows(const PagedAttnDev& p, int hk, int row0, int rows, int x0, int stride, int c,
+                                                int last, int lane) {
   constexpr int kVec = D / 32;
-  for (int x = (threadIdx.x >> 5) * gridDim.y + blockIdx.y; x < rows; x += 8 * gridDim.y) {
-    const int tok = x / p.G, h = hk * p.G + (x - tok * p.G);
-    const int t = tok >= p.tile_tokens ? 1 : 0;
-    const int r = t * kBM + x - t * p.tile_tokens * p.G;     // row inside the parts
-    auto row_of = [&](int cc) { return (cc == c - 1 ? 2LL * cc + 1 : 2LL * cc) * 256 + r; };
-    // log2 sum of CTA cc's part; -inf: it has none (its share of the line holds the start of no tile)
-    auto part = [&](int cc) {
-      return cc < c || tile_at(cc) < min(b.y, tile_at(cc + 1)) ? __ldcg(p.part_lse + row_of(cc)) : -INFINITY;
-    };
-    float m = -INFINITY;
-    for (int cc = c - 1 + lane; cc <= last; cc += 32) m = fmaxf(m, part(cc));
+  const int row_tile = p.tile_tokens * p.G;
+  int row[kRows];                   // inside a part
+  float m[kRows], acc[kRows][kVec], sum[kRows];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    float acc[kVec], sum = 0.f;
+  for (int k = 0; k < kRows; ++k) {
+    const int x = min(x0 + k * stride, rows - 1);        // a row too many is computed again and not written
+    row[k] = x < row_tile ? x : kBM + x - row_tile;
+    m[k] = -INFINITY;
+    sum[k] = 0.f;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) acc[k] = 0.f;
-    if (m > -INFINITY) {
-#pragma unroll 4
-      for (int cc = c - 1; cc <= last; ++cc) {
-        const float lse = part(cc);
-        if (lse == -INFINITY) continue;
-        const float wgt = ex2_approx(lse - m);
-        const float* src = p.part_o + row_of(cc) * D + lane * kVec;
-        sum += wgt;
-        if constexpr (kVec == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] = fmaf(wgt, v.x, acc[0]);
-          acc[1] = fmaf(wgt, v.y, acc[1]);
-          acc[2] = fmaf(wgt, v.z, acc[2]);
-          acc[3] = fmaf(wgt, v.w, acc[3]);
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] = fmaf(wgt, v.x, acc[0]);
-          acc[1] = fmaf(wgt, v.y, acc[1]);
+    for (int e = 0; e < kVec; ++e) acc[k][e] = 0.f;
+  }
+  for (int base = c - 1; base <= last; base += 32) {
+    // a CTA without a tile of its own (its start is the next one's) has no part; the first one, c - 1, always has
+    bool here = base + lane <= last;
+    if (here && base + lane >= c) {
+      const int4 from = paged_start_of(p.work, base + lane), to = paged_start_of(p.work, base + lane + 1);
+      here = from.x != to.x || from.y != to.y || from.z != to.z;
+    }
+    unsigned parts = __ballot_sync(0xffffffffu, here);
+    while (parts) {
+      float lse[kParts][kRows], v[kParts][kRows][kVec];
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) {
+        const bool any = parts != 0;
+        const int cc = any ? base + __ffs(parts) - 1 : c - 1;
+        if (any) parts &= parts - 1;
+        // part c - 1 is its CTA's last stretch, the others are first ones
+        const long long slot = (cc == c - 1 ? 2LL * cc + 1 : 2LL * cc) * 256;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          lse[q][k] = any ? __ldcg(p.part_lse + slot + row[k]) : -INFINITY;
+          const float* src = p.part_o + (slot + row[k]) * D + lane * kVec;
+          if constexpr (kVec == 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
+            v[q][k][0] = f.x; v[q][k][1] = f.y; v[q][k][2] = f.z; v[q][k][3] = f.w;
+          } else {
+            const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
+            v[q][k][0] = f.x; v[q][k][1] = f.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) {
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          if (lse[q][k] == -INFINITY) continue;       // no part, or the row sees none of its keys
+          const float top = fmaxf(m[k], lse[q][k]);
+          const float keep = ex2_approx(m[k] - top), wgt = ex2_approx(lse[q][k] - top);
+          m[k] = top;
+          sum[k] = sum[k] * keep + wgt;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) acc[k][e] = fmaf(acc[k][e], keep, wgt * v[q][k][e]);
         }
       }
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    const long long token = a.x + tok;
-    if (p.lse && lane == 0) p.lse[token * p.Hq + h] = sum > 0.f ? (m + lg2_approx(sum)) * kLn2 : -INFINITY;
+  }
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const int x = x0 + k * stride;
+    if (x >= rows) break;
+    const int tok = x / p.G, h = hk * p.G + (x - tok * p.G);
+    const float inv = sum[k] > 0.f ? 1.f / sum[k] : 0.f;
+    const long long token = row0 + tok;
+    if (p.lse && lane == 0) p.lse[token * p.Hq + h] = sum[k] > 0.f ? (m[k] + lg2_approx(sum[k])) * kLn2 : -INFINITY;
     const int col = lane * kVec, in = col & 63;
     if (in < p.blk) {
       uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + token * p.out_st + h * p.out_sh + (col >> 6) * p.blk + in);
 #pragma unroll
-      for (int k = 0; k < kVec; k += 2) dst[k >> 1] = pack2<kBf16>(acc[k] * inv, acc[k + 1] * inv);
+      for (int e = 0; e < kVec; e += 2) dst[e >> 1] = pack2<kBf16>(acc[k][e] * inv, acc[k][e + 1] * inv);
     }
+  }
+}
+
+// Joins the partial rows of an item cut by CTA borders: with the parts' log2 sums L_c,
+//   out = sum_c 2^(L_c - L) o_c,   L = log2 sum_c 2^L_c,
+// in the order of the keys. Block (c, y) looks at the start of CTA c + 1 and works iff that is the first border inside its
+// item; rows are dealt over the y blocks and their warps. Each partial row is read once. It is launched while the main
+// kernel still runs (programmatic dependent launch) and waits for its results only after it has found its item.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256)
+paged_combine_kernel(const PagedAttnDev p) {
+  const int ctas = __ldg(p.work + 1), c = blockIdx.x + 1, lane = threadIdx.x & 31;
+  int last = c;                       // last CTA with a part of the item
+  bool first_inside = false;
+  int4 a = make_int4(0, 0, 0, 0), at = a;
+  if (c < ctas) {
+    at = paged_start_of(p.work, c);
+    const int4 before = paged_start_of(p.work, c - 1);
+    first_inside = at.z > 0 && !(before.x == at.x && before.y == at.y && before.z > 0);
+    if (first_inside) {
+      a = __ldg(reinterpret_cast<const int4*>(p.work + p.items_at) + 2 * static_cast<long long>(at.y));
+      while (true) {
+        const int cc = last + 1 + lane;
+        bool same = false;
+        if (cc < ctas) {
+          const int4 x = paged_start_of(p.work, cc);
+          same = x.x == at.x && x.y == at.y;
+        }
+        const unsigned votes = __ballot_sync(0xffffffffu, same);
+        const int n = votes == 0xffffffffu ? 32 : __ffs(~votes) - 1;
+        last += n;
+        if (n < 32) break;
+      }
+    }
+  }
+  // (every block waits, so that this kernel never ends before the main one)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!first_inside) return;
+  const int rows = a.y * p.G, stride = 8 * gridDim.y;
+  int x = (threadIdx.x >> 5) + 8 * blockIdx.y;
+  if (rows <= stride) {
+    if (x < rows) paged_join_rows<D, kBf16, 1, 8>(p, at.x, a.x, rows, x, stride, c, last, lane);
+  } else {
+    for (; x < rows; x += 4 * stride) paged_join_rows<D, kBf16, 4, 2>(p, at.x, a.x, rows, x, stride, c, last, lane);
   }
 }
 
@@ -704,7 +689,7 @@ static cudaError_t launch_paged_one(const PagedAttnLaunch& a, cudaStream_t strea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, kBf16>, a.p, grid);
+  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, kBf16>, a.p);
 }
 
 template <int D>

@@ -6,7 +6,12 @@
 //   fresh_b = sum over the requests before b of need - have: its pages in the list of free ones start there
 //   token i of it: position c_b + i, slot = page(position >> s) * 2^s + position mod 2^s
 // and the work list of the attention: items of `item_tokens` query tokens with the number of 128-key tiles that each
-// of them sees, what a tile costs (2 if the tokens need both query tiles, else 1) and the cost of the items before it.
+// of them sees and what such a tile costs (2 if the tokens need both query tiles, else 1). All tiles of all items of all
+// key/value heads form a line as long as their costs (an item begins with the cost of two of its tiles, which is what
+// its start and its end take), which is cut into equal shares, one per SM. A border that falls next to
+// an end of an item moves to that end, by at most snap_of (and half a share): an item that is cut costs partial rows of both
+// sides, written and joined, about as much as two tiles of 256 rows or half a tile of a few.
+// (36 x 4 items of two tiles and 256 rows, D = 64: SNAP0 us with every border where it falls, SNAP1 us with moved ones.)
 //
 // One launch. Every block scans the requests by itself in shared memory (a few thousand numbers: cheaper than a second
 // launch that waits for the first), then block 0 writes the work list while the others place tokens, one per thread.
@@ -50,6 +55,9 @@ __device__ __forceinline__ T block_exclusive(T v, T* warp_tot, T& total) {
   __syncthreads();      // warp_tot may be used again
   return before + x - v;
 }
+
+// How far a border may move, by the cost of the item's tiles.
+__device__ __forceinline__ int snap_of(int cost) { return cost == 2 ? 4 : 1; }
 
 // Largest index r in [0, n) with a[r] <= x (a ascends, a[0] <= x).
 __device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
@@ -141,7 +149,7 @@ paged_plan_kernel(const PagedPlanDev p) {
   }
   __syncthreads();
   long long carry = 0;
-  int4* items = reinterpret_cast<int4*>(p.work + kWorkHeader);
+  int4* items = reinterpret_cast<int4*>(p.work + p.items_at);
   for (int base = 0; base < n_items; base += kPlanThreads) {
     const int i = base + tid;
     int4 a = make_int4(0, 0, 0, 0);
@@ -157,16 +165,45 @@ paged_plan_kernel(const PagedPlanDev p) {
       cost = 2 * n > p.item_tokens ? 2 : 1;
     }
     long long all;
-    const long long before = carry + block_exclusive(tiles * cost, warp_tot, all);
+    const long long before = carry + block_exclusive(i < n_items ? (tiles + 2) * cost : 0LL, warp_tot, all);
     if (i < n_items) {
       items[2 * i] = a;
       items[2 * i + 1] = make_int4(static_cast<int>(before), static_cast<int>(tiles), cost, 0);
     }
     carry += all;
   }
+  // ---- shares (the items written above are visible to the block behind the barrier)
+  __syncthreads();
+  const long long per_head = carry, line = per_head * p.heads_kv;
+  const int ctas = static_cast<int>(min(line, static_cast<long long>(p.sms)));
   if (tid == 0) {
     p.work[0] = n_items;
-    p.work[1] = static_cast<int>(carry);
+    p.work[1] = ctas;
+  }
+  if (ctas == 0) return;
+  const long long share = line / ctas, extra = line - share * ctas;
+  const int* prefix = p.work + p.items_at + 4;
+  for (int c = tid; c <= ctas; c += kPlanThreads) {
+    int4 start = make_int4(p.heads_kv, 0, 0, 0);
+    if (c < ctas) {
+      const long long g = share * c + min(static_cast<long long>(c), extra);
+      const int hk = static_cast<int>(g / per_head);
+      const int rem = static_cast<int>(g - hk * per_head);
+      int lo = 0, hi = n_items;      // the item with the largest prefix not above rem
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[static_cast<long long>(mid) * kWorkItem] <= rem) lo = mid; else hi = mid;
+      }
+      const int4 item = items[2 * static_cast<long long>(lo) + 1];
+      const int cost = item.z, in = max(0, rem - item.x - 2 * cost), left = item.y * cost - in;
+      const int snap = static_cast<int>(min(static_cast<long long>(snap_of(cost)), share >> 1));
+      int tile = (in + cost - 1) / cost;
+      if (in <= snap && in <= left) tile = 0;
+      else if (left <= snap) tile = item.y;
+      start = make_int4(hk, lo, tile, 0);
+      if (tile >= item.y) start = lo + 1 < n_items ? make_int4(hk, lo + 1, 0, 0) : make_int4(hk + 1, 0, 0, 0);
+    }
+    reinterpret_cast<int4*>(p.work + kWorkHeader)[c] = start;
   }
 }
 

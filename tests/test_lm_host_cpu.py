@@ -181,8 +181,10 @@ def test_plan_refusals(change, code, word):
 
 def test_paged_sizes():
     lib = _capi.load()
-    assert lib.fa2_paged_work_bytes(3, 100, 8, 2) == 4 * (16 + 8 * (100 // 64 + 3))      # 64 tokens of 4 heads per item
-    assert lib.fa2_paged_work_bytes(200, 100, 8, 8) == 4 * (16 + 8 * 100)                # at most one item per token
+    sms = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148
+    head = 16 + (4 * (sms + 1) + 7) // 8 * 8                                             # header and the CTAs' starts
+    assert lib.fa2_paged_work_bytes(3, 100, 8, 2) == 4 * (head + 8 * (100 // 64 + 3))    # 64 tokens of 4 heads per item
+    assert lib.fa2_paged_work_bytes(200, 100, 8, 8) == 4 * (head + 8 * 100)              # at most one item per token
     assert lib.fa2_paged_work_bytes(3, 100, 3, 2) == 0
     assert lib.fa2_paged_workspace_bytes(256) == 0 and lib.fa2_paged_workspace_bytes(20) == 0
     assert lib.fa2_paged_workspace_bytes(128) % (2 * 256 * 129 * 4) == 0

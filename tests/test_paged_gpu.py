@@ -95,10 +95,19 @@ def test_work_list_covers_every_token_once(heads_q, heads_kv):
             tiles = -(-(c + t + m) // 128)
             cost = 2 if 2 * m > per else 1      # a tile of an item that fills both query tiles counts twice
             want.append([sum(new[:b]) + t, m, c + t, b, before, tiles, cost, 0])
-            before += cost * tiles
+            before += cost * (tiles + 2)        # and an item costs two tiles more than it has
     work = plan.work.tolist()
-    assert work[:2] == [len(want), before]
-    assert work[16:16 + 8 * len(want)] == [x for w in want for x in w]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    at = 16 + (4 * (sms + 1) + 7) // 8 * 8
+    assert work[:2] == [len(want), min(sms, before * heads_kv)]
+    assert work[at:at + 8 * len(want)] == [x for w in want for x in w]
+    # the CTAs' starts go through every tile of every item and head once, in order
+    starts = [tuple(work[16 + 4 * c:19 + 4 * c]) for c in range(work[1] + 1)]
+    assert starts[0] == (0, 0, 0) and starts[-1] == (heads_kv, 0, 0) and starts == sorted(starts)
+    assert all(tile < want[item][5] for _, item, tile in starts[:-1])
+    share = before * heads_kv / work[1]
+    cost = lambda s: s[0] * before + (want[s[1]][4] + (s[2] + 2 * (s[2] > 0)) * want[s[1]][6] if s[0] < heads_kv else 0)
+    assert all(cost(b) - cost(a) <= share + 2 * (4 + 4) + 2 for a, b in zip(starts, starts[1:]))
 
 
 def test_plan_without_enough_pages_width_or_rows():
