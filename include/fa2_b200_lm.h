@@ -46,8 +46,8 @@ typedef struct {
 size_t fa2_document_layout_bytes(int32_t batch, int32_t seqlen);
 
 /* Reads document ids (int32, rows `stride_b` elements apart) and writes the layout that the two calls
- * below take: for every token the first and one past the last token of its document, and the same over
- * every 128 tokens. `layout`: 16-byte aligned, fa2_document_layout_bytes. One layout serves the forward
+ * below take: for every token the first and one past the last token of its document, the same over
+ * every 128 tokens, and an order of work. `layout`: 16-byte aligned, fa2_document_layout_bytes. One layout serves the forward
  * and backward calls of every layer that works on these rows. */
 int fa2_document_layout(const int32_t* document_ids, int64_t stride_b, int32_t batch, int32_t seqlen,
                         int32_t* layout, size_t layout_bytes, void* cuda_stream);

@@ -330,9 +330,11 @@ bool can_pack_heads(const fa2_problem& p) {
   return p.seqlen_q == 1 && group > 1 && group <= 128 && !(p.dropout_p > 0.f);
 }
 
-// Sizes and parts of a document layout (int32): token bounds [B][S] twice, tile bounds [B][ceil(S/128)] twice.
+// Sizes and parts of a document layout (int32): token bounds [B][S] twice, tile bounds [B][ceil(S/128)] twice, order of the
+// blocks of 256 rows [B * ceil(S/256)].
 size_t document_layout_ints(int64_t batch, int64_t seqlen) {
-  return static_cast<size_t>(batch) * (2 * static_cast<size_t>(seqlen) + 2 * ((static_cast<size_t>(seqlen) + 127) / 128));
+  const size_t s = static_cast<size_t>(seqlen);
+  return static_cast<size_t>(batch) * (2 * s + 2 * ((s + 127) / 128) + (s + 255) / 256);
 }
 
 constexpr float kMinSoftcap = 1.f / 1024.f, kMaxSoftcap = 1024.f;
@@ -375,6 +377,7 @@ int make_score_mod(ScoreModDev* out, int* mode, const fa2_score_mod& m, const fa
     out->tok_hi = out->tok_lo + tokens;
     out->tile_lo = out->tok_hi + tokens;
     out->tile_hi = out->tile_lo + tiles;
+    out->order = out->tile_hi + tiles;
   }
   if (m.o_rest) {
     if (reinterpret_cast<uintptr_t>(m.o_rest) & 15) return fail(FA2_ERR_UNSUPPORTED, "o_rest must be 16-byte aligned");
@@ -541,6 +544,8 @@ int fa2_document_layout(const int32_t* document_ids, int64_t stride_b, int32_t b
   if (reinterpret_cast<uintptr_t>(document_ids) & 3)
     return fail(FA2_ERR_INVALID_ARG, "document_ids must be 4-byte aligned");
   if (reinterpret_cast<uintptr_t>(layout) & 15) return fail(FA2_ERR_INVALID_ARG, "layout must be 16-byte aligned");
+  if (static_cast<int64_t>(batch) * ((seqlen + 255) / 256) > INT_MAX)
+    return fail(FA2_ERR_UNSUPPORTED, "batch * seqlen is too large");
   const size_t need = document_layout_ints(batch, seqlen) * sizeof(int32_t);
   if (layout_bytes < need) return fail(FA2_ERR_INVALID_ARG, "layout must hold %zu bytes", need);
   const cudaError_t e =

@@ -121,10 +121,58 @@ document_layout_kernel(const int* __restrict__ ids, long long stride_b, int B, i
   }
 }
 
+// Order in which the forward takes the blocks of 256 query rows: by the key tiles they walk over, longest first (as the
+// forward deals them out in rounds of alternating direction, that evens out the SMs' shares: 4 rows of 4096 tokens with
+// documents of 700 on average, 32 heads, 148 SMs: longest share 231 tiles in the order of the rows, 191 sorted, mean 189).
+// The walk ends at the block's own last key, as under causal masking. A counting sort by one block; blocks of equal length
+// land in any order, which changes no result.
+constexpr int kOrderBins = 2048;
+__global__ void __launch_bounds__(kLayoutThreads)
+document_order_kernel(int B, int S, int* __restrict__ layout) {
+  __shared__ int bins[kOrderBins];
+  __shared__ int warp_tot[32];
+  const long long BS = static_cast<long long>(B) * S;
+  const int nt = (S + 127) >> 7, nq = (S + 255) >> 8, n = B * nq, tid = threadIdx.x;
+  const int* tile_lo = layout + 2 * BS;
+  const int* tile_hi = tile_lo + static_cast<long long>(B) * nt;
+  int* order = layout + 2 * BS + 2 * static_cast<long long>(B) * nt;
+  // bin of a block: 0 for the longest
+  auto bin = [&](int i) {
+    const int b = i / nq, q = i - b * nq;
+    int first = INT_MAX, end = 0;
+    for (int t = 2 * q; t < min(nt, 2 * q + 2); ++t) {
+      const long long at = static_cast<long long>(b) * nt + t;
+      const int hi = min(tile_hi[at], min(S, t * 128 + 128));
+      if (hi > tile_lo[at]) {
+        first = min(first, tile_lo[at]);
+        end = max(end, hi);
+      }
+    }
+    const int len = end > 0 ? ((end + 127) >> 7) - (first >> 7) : 0;
+    return kOrderBins - 1 - min(len, kOrderBins - 1);
+  };
+  for (int k = tid; k < kOrderBins; k += kLayoutThreads) bins[k] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kLayoutThreads) atomicAdd(bins + bin(i), 1);
+  __syncthreads();
+  // exclusive sum over the bins, two per thread
+  const int own0 = bins[2 * tid], own1 = bins[2 * tid + 1];
+  const int incl = block_scan<false>(own0 + own1, [](int x, int y) { return x + y; }, warp_tot);
+  __syncthreads();
+  bins[2 * tid] = incl - own0 - own1;
+  bins[2 * tid + 1] = incl - own1;
+  __syncthreads();
+  for (int i = tid; i < n; i += kLayoutThreads) order[atomicAdd(bins + bin(i), 1)] = i;
+}
+static_assert(kOrderBins == 2 * kLayoutThreads, "two bins per thread");
+
 }  // namespace
 
 cudaError_t launch_document_layout(const int* ids, long long stride_b, int B, int S, int* layout, cudaStream_t stream) {
   document_layout_kernel<<<static_cast<unsigned>(B), kLayoutThreads, 0, stream>>>(ids, stride_b, B, S, layout);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  document_order_kernel<<<1, kLayoutThreads, 0, stream>>>(B, S, layout);
   return cudaGetLastError();
 }
 

@@ -64,7 +64,9 @@ struct FwdSmem {
   static constexpr int kNumBarsBase = 4 + 2 * kStages + 2 + 2 * kPSplit + 4;
   static constexpr int kNumBars = kNumBarsBase + (kStaged ? 8 * kTermSlots : 0);
   static constexpr int kMiscOff = kBarOff + kNumBars * 8;
-  static constexpr int kTotal = kMiscOff + 16;
+  // scored kernels, per softmax warp: what it needs again behind its loop over the key tiles
+  static constexpr int kNoteOff = kMiscOff + 16;
+  static constexpr int kTotal = kNoteOff + (kStaged ? 0 : 8 * 16);
   static constexpr int kDynamicBytes = kTotal + 1024;  // room to align the base to 1024 B
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
 };
@@ -75,6 +77,7 @@ struct FwdItem {
   int split, j0;   // split-KV: which part of the K/V sequence, and its first tile
   int sq, sk;   // rows of this batch element that take part (the problem's, or its seqlens entry)
   int n_tiles[kTilesPerCta];
+  int first[kTilesPerCta];   // scored kernels: key tiles of the stream before the first one this query tile sees
   int n_max;
 };
 
@@ -91,9 +94,19 @@ __device__ __forceinline__ void decode_item(const FwdKernelParams& p, int w, Fwd
   const int bh = w - qb_rank * nbh;
   // causal: the longest blocks come first
   const bool longest_first = kMod == kNoMod ? kCausal : p.mod.causal != 0;
-  const int qblk = longest_first ? (p.n_qblk - 1 - qb_rank) : qb_rank;
+  int qblk = longest_first ? (p.n_qblk - 1 - qb_rank) : qb_rank;
   it.b = bh / p.Hq;
   it.h = bh - it.b * p.Hq;
+  if constexpr (kMod != kNoMod) {
+    if (p.mod.order != nullptr) {
+      // packed documents: how long a block of rows is depends on where its documents begin, so the layout has sorted them
+      const int rank = w / p.Hq;
+      const int at = __ldg(p.mod.order + rank);
+      it.h = w - rank * p.Hq;
+      it.b = at / p.n_qblk;
+      qblk = at - it.b * p.n_qblk;
+    }
+  }
   it.hk = it.h / p.G;
   it.q0 = qblk * (kBM * kTilesPerCta);
   it.sq = p.Sq;
@@ -104,8 +117,7 @@ __device__ __forceinline__ void decode_item(const FwdKernelParams& p, int w, Fwd
     it.sk = min(len, p.Sk);
   }
   if constexpr (kMod != kNoMod) {
-    // Both query tiles walk one stream of key tiles, which begins at the first tile either of them sees (a tile
-    // that one of them does not see is masked for it).
+    // Both query tiles walk one stream of key tiles, which begins at the first tile either of them sees.
     int lo[kTilesPerCta], hi[kTilesPerCta], first = 0x7fffffff;
 #pragma unroll
     for (int t = 0; t < kTilesPerCta; ++t) {
@@ -118,7 +130,10 @@ __device__ __forceinline__ void decode_item(const FwdKernelParams& p, int w, Fwd
     }
     it.j0 = first == 0x7fffffff ? 0 : first;
 #pragma unroll
-    for (int t = 0; t < kTilesPerCta; ++t) it.n_tiles[t] = hi[t] > lo[t] ? hi[t] - it.j0 : 0;
+    for (int t = 0; t < kTilesPerCta; ++t) {
+      it.n_tiles[t] = max(0, hi[t] - lo[t]);
+      it.first[t] = it.n_tiles[t] > 0 ? lo[t] - it.j0 : 0;
+    }
   } else {
 #pragma unroll
     for (int t = 0; t < kTilesPerCta; ++t) {
@@ -136,6 +151,7 @@ __device__ __forceinline__ void decode_item(const FwdKernelParams& p, int w, Fwd
     }
   }
   it.n_max = max(it.n_tiles[0], it.n_tiles[1]);
+  if constexpr (kMod != kNoMod) it.n_max = max(it.first[0] + it.n_tiles[0], it.first[1] + it.n_tiles[1]);
 }
 
 }  // namespace
@@ -316,6 +332,53 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
           }
         }
         if (!ok || it.n_max == 0) continue;
+        if constexpr (kScored) {
+          // the same steps as below for query tiles that may begin later in the stream: O_t += P_t V_j, then S_t of the next
+          // key tile, for every query tile that sees them
+          for (int j = -1; j < it.n_max && ok; ++j) {
+            const bool has_next = j + 1 < it.n_max;
+            int slot_v = 0, slot_k = 0;
+            if (j >= 0) {
+              slot_v = kv_count % L::kStages;
+              ok = mbar_wait_warp(bar_kv_full(slot_v), (kv_count / L::kStages) & 1u, abort_flag);
+              ++kv_count;
+            }
+            if (ok && has_next) {
+              slot_k = kv_count % L::kStages;
+              ok = mbar_wait_warp(bar_kv_full(slot_k), (kv_count / L::kStages) & 1u, abort_flag);
+              ++kv_count;
+            }
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int t = 0; t < kTilesPerCta; ++t) {
+              const int first = it.first[t], end = first + it.n_tiles[t];
+              const bool pv = j >= first && j < end;
+              if (pv) {
+                // (the epilogue of the previous item has read O_t out of tensor memory)
+                if (j == first) ok = mbar_wait_warp(bar_o_free(t), (item_idx & 1u) ^ 1u, abort_flag);
+#pragma unroll
+                for (int hh = 0; hh < kPSplit; ++hh) {
+                  if (ok) ok = mbar_wait_warp(bar_p_full(t, hh), it_cnt[t] & 1u, abort_flag);
+                  if (!ok) break;
+                  tc_fence_after();
+                  issue_o(t, slot_v, j == first, hh);
+                }
+                if (!ok) break;
+                ++it_cnt[t];
+              }
+              if (j + 1 >= first && j + 1 < end) {
+                issue_s(t, slot_k);
+                if (j + 2 == end) mma_commit_e(bar_q_free(t));   // last S of tile t issued
+              }
+              if (pv && j + 1 == end) mma_commit_e(bar_o_full(t));
+            }
+            if (!ok) break;
+            if (j >= 0) mma_commit_e(bar_kv_empty(slot_v));
+            if (has_next) mma_commit_e(bar_kv_empty(slot_k));
+          }
+          continue;
+        }
         {
           const int slot = kv_count % L::kStages;
           ok = mbar_wait_warp(bar_kv_full(slot), (kv_count / L::kStages) & 1u, abort_flag);
@@ -401,11 +464,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     for (int w = first_item(); w < total_items; w = next_item(w)) {
       FwdItem it;
       decode_item<kCausal, kMod>(p, w, it);
-      const int b = it.b, h = it.h;
-      const int b_out = it.b + it.split * p.B;   // where this item's output and lse go
-      const int qi = it.q0 + t * kBM + r;      // global query row
+      int b = it.b, h = it.h;
+      int b_out = it.b + it.split * p.B;       // where this item's output and lse go
+      int qi = it.q0 + t * kBM + r;            // global query row
       const int nt = it.n_tiles[t];
-      const bool tile_valid = (it.q0 + t * kBM) < p.Sq;
+      bool tile_valid = (it.q0 + t * kBM) < p.Sq;
       // last visible key of this row (none for rows past the end of the sequence)
       const int row_lim =
           qi < it.sq ? (kCausal ? min(it.sk - 1, qi + p.causal_off) : it.sk - 1) : -1;
@@ -491,13 +554,31 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         if (qi < p.Sq) query_interval(p.mod, b, qi, p.Sq, p.Sk, p.causal_off, lo, hi);
         const ModTerms<kMod> terms(p.scale_log2, p.mod.arg2, p.mod.cap2, has_slope(kMod) ? __ldg(p.mod.slopes + h) : 0.f,
                                    qi + p.causal_off);
+        const int tile0 = it.j0 + it.first[t];
+        // In the loop a row's 128 scores leave no registers for the item: it is noted down meanwhile (see PagedNote).
+        volatile int* note = reinterpret_cast<volatile int*>(smem_gen + L::kNoteOff + warp * 16);
+        if (lane == 0) {
+          note[0] = w;
+          note[1] = b_out;
+          note[2] = h;
+          note[3] = it.q0;
+        }
+        __syncwarp();
         for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
           ok = mbar_wait(bar_s_full(t), it_cnt & 1u, abort_flag);
           if (!ok) break;
-          softmax_tile_row<D, kBf16, false, true, kBf16>(tS, tO, it.j0 + j, j > 0, p, hi - 1, sc, false, m, l, [] {},
+          softmax_tile_row<D, kBf16, false, true, kBf16>(tS, tO, tile0 + j, j > 0, p, hi - 1, sc, false, m, l, [] {},
                                                          [&](int hh) { mbar_arrive(bar_p_full(t, hh)); }, terms, keep,
                                                          lo, &l16);
         }
+        w = note[0];
+        b_out = note[1];
+        h = note[2];
+        it.q0 = note[3];
+        b = b_out % p.B;
+        qi = it.q0 + t * kBM + r;
+        tile_valid = (it.q0 + t * kBM) < p.Sq;
+        __syncwarp();
       } else {
         for (int j = 0; j < nt && ok; ++j, ++it_cnt) {
           ok = mbar_wait(bar_s_full(t), it_cnt & 1u, abort_flag);

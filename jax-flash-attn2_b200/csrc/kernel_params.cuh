@@ -78,6 +78,7 @@ struct ScoreModDev {
   // (0, 0 for padding), and the same over every 128 tokens (least first, greatest end)
   const int *tok_lo, *tok_hi;     // [B][Sq]
   const int *tile_lo, *tile_hi;   // [B][ceil(Sq / 128)]
+  const int* order;               // [B * ceil(Sq / 256)]: blocks of 256 rows (b * ceil(Sq / 256) + block), longest first
   // What the rounding of the output to 16 bits dropped, itself in 16 bits, or null: written by the forward and added
   // to the output again where the backward forms rowsum(o * do). Element strides.
   uint16_t* rest;

@@ -122,17 +122,18 @@ __device__ __forceinline__ int key_tiles_above(const ScoreModDev& m, int b, int 
 
 // tanh(z) of N values of a row, z = ln2 / 2 * arg2 * x (that is, e^(2z) = 2^(arg2 x)), in place. All 32 lanes call it.
 //
-// Where every |z| of the warp's values is at most 1 (scores below the cap, which is what a cap is chosen for), it is an odd
-// polynomial, z times a polynomial of degree 5 in z^2 that is best in the maximum norm (found by weighted least squares
-// repeated until the error levels out): |error| <= 2.4e-7, fused multiply-adds of pairs alone. Otherwise 1 - 2 r with
-// r = 1 / (1 + 2^(arg2 x)): an exponential and a reciprocal, |error| <= 2^-22. A cap of 50 turns either into at most 2^-15
-// in the exponent of a weight, far below the 2^-9 of the rounding of P; the hardware's tanh (2^-11 relative) would move the
-// weights by percents. The special functions are what a capped kernel would be bound by otherwise: 16 lanes per cycle and SM,
-// three per score. Measured (2 x 8192 causal, 32/8 heads, D = 128, cap 50): forward 1.96 ms with the second form alone,
-// 2.00 with a polynomial in 2^-|arg2 x| instead of the reciprocal, 1.70 ms as it is; backward 3.61, 3.84, 3.54 ms.
-constexpr float kSmallTanh = 2.8853900817779268f;   // 2 log2(e): |arg2 x| at |z| = 1
-constexpr float kT0 = 0.34657249991665245f, kT1 = -0.013872143458246167f, kT2 = 0.0006626874361558277f,
-                kT3 = -3.061309816091965e-05f, kT4 = 1.1624315928559195e-06f, kT5 = -2.4602920433007444e-08f;
+// Where every |z| of the warp's values is at most 3/4 (scores well below the cap, which is what a cap is chosen for), it is an
+// odd polynomial, z times a polynomial of degree 4 in z^2 that is best in the maximum norm (found by weighted least squares
+// repeated until the error levels out): |error| <= 2e-7, fused multiply-adds of pairs alone, with the scale of x in the
+// coefficients. Otherwise 1 - 2 r with r = 1 / (1 + 2^(arg2 x)): an exponential and a reciprocal, |error| <= 2^-22. A cap of
+// 50 turns either into at most 2^-15 in the exponent of a weight, far below the 2^-9 of the rounding of P; the hardware's
+// tanh (2^-11 relative) would move the weights by percents. The special functions are what a capped kernel would be bound by
+// otherwise: 16 lanes per cycle and SM, three per score. Measured (2 x 8192 causal, 32/8 heads, D = 128, cap 50): forward
+// 1.96 ms with the second form alone, 2.00 with a polynomial in 2^-|arg2 x| instead of the reciprocal, 1.68 with the first
+// form up to |z| = 1 (one degree more), 1.55 ms as it is; backward 3.61, 3.84, 3.50, 3.25 ms.
+constexpr float kSmallTanh = 2.1640425613334453f;   // 1.5 log2(e): |arg2 x| at |z| = 3/4
+constexpr float kT0 = 0.9999972283219466f, kT1 = -0.333230764880115f, kT2 = 0.1322609166463934f,
+                kT3 = -0.04928044841513475f, kT4 = 0.012318832984223586f;
 template <int N>
 __device__ __forceinline__ void tanh_row(float (&x)[N], float arg2) {
   float a0 = 0.f, a1 = 0.f;
@@ -141,18 +142,20 @@ __device__ __forceinline__ void tanh_row(float (&x)[N], float arg2) {
     a0 = max3(a0, fabsf(x[c]), fabsf(x[c + 1]));
     a1 = max3(a1, fabsf(x[c + 2]), fabsf(x[c + 3]));
   }
-  if (!__any_sync(0xffffffffu, fmaxf(a0, a1) * arg2 > kSmallTanh)) {
+  const float z1 = arg2 * 0.34657359027997264f, z2 = z1 * z1;       // z = z1 x
+  // (beyond z1 = 2^13 the last coefficient would leave the range of float32)
+  if (z1 < 8192.f && !__any_sync(0xffffffffu, fmaxf(a0, a1) * arg2 > kSmallTanh)) {
+    const float c0 = kT0 * z1, c1 = kT1 * (z1 * z2), c2 = kT2 * (z1 * z2 * z2), c3 = kT3 * (z1 * z2 * z2 * z2),
+                c4 = kT4 * (z1 * z2 * z2 * (z2 * z2));
 #pragma unroll
     for (int c = 0; c < N; c += 2) {
-      float y0, y1, u0, u1, t0, t1;
-      fma2(y0, y1, x[c], x[c + 1], arg2, arg2, 0.f, 0.f);
-      fma2(u0, u1, y0, y1, y0, y1, 0.f, 0.f);
-      fma2(t0, t1, u0, u1, kT5, kT5, kT4, kT4);
-      fma2(t0, t1, t0, t1, u0, u1, kT3, kT3);
-      fma2(t0, t1, t0, t1, u0, u1, kT2, kT2);
-      fma2(t0, t1, t0, t1, u0, u1, kT1, kT1);
-      fma2(t0, t1, t0, t1, u0, u1, kT0, kT0);
-      fma2(x[c], x[c + 1], t0, t1, y0, y1, 0.f, 0.f);
+      float u0, u1, t0, t1;
+      fma2(u0, u1, x[c], x[c + 1], x[c], x[c + 1], 0.f, 0.f);
+      fma2(t0, t1, u0, u1, c4, c4, c3, c3);
+      fma2(t0, t1, t0, t1, u0, u1, c2, c2);
+      fma2(t0, t1, t0, t1, u0, u1, c1, c1);
+      fma2(t0, t1, t0, t1, u0, u1, c0, c0);
+      fma2(x[c], x[c + 1], t0, t1, x[c], x[c + 1], 0.f, 0.f);
     }
   } else {
 #pragma unroll

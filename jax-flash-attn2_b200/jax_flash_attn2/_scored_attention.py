@@ -95,7 +95,7 @@ def _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest=No
     if layout is not None:
         if k.shape[1] != sq:
             raise ValueError("documents need as many keys as queries")
-        need = batch * (2 * sq + 2 * ((sq + 127) // 128))
+        need = batch * (2 * sq + 2 * ((sq + 127) // 128) + (sq + 255) // 256)
         if layout.dtype != torch.int32 or layout.numel() != need or not layout.is_contiguous() or layout.device != q.device:
             raise ValueError("layout must be what document_layout returned for ids of shape "
                              f"[{batch}, {sq}] on the device of q")

@@ -90,7 +90,7 @@ def test_combinations_that_are_not_offered_are_refused():
 
 def test_document_layout_arguments():
     lib = _capi.load()
-    assert lib.fa2_document_layout_bytes(3, 130) == 4 * 3 * (2 * 130 + 2 * 2)
+    assert lib.fa2_document_layout_bytes(3, 130) == 4 * 3 * (2 * 130 + 2 * 2 + 1)
     assert lib.fa2_document_layout_bytes(0, 130) == 0
     need = lib.fa2_document_layout_bytes(3, 130)
     call = lambda ids=0x1000, stride=130, b=3, s=130, out=0x2000, n=need: lib.fa2_document_layout(ids, stride, b, s, out, n, None)

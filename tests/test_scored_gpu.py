@@ -118,6 +118,32 @@ def test_storage_with_heads_before_rows(D):
     check(2, 200, 200, 4, 2, D, BF16, True, sharp=2.0, cap=10.0, slopes=slopes_of(4), transposed=True)
 
 
+def test_zeros_under_a_tiny_cap_and_a_large_scale():
+    # scores of exactly 0 where scale / cap is beyond what the polynomial's coefficients can hold
+    import jax_flash_attn2 as J
+    k, v = (x.cuda() for x in W.make_qkv(1, 64, 64, 1, 1, 64, BF16)[1:3])
+    for scale in (1e6, 1e30):
+        out = J.scored_flash_attention(torch.zeros_like(k), k, v, scale, False, softcap=2.0 ** -10)
+        want = v.float().mean(1, keepdim=True).expand_as(v)
+        assert torch.all((out.float() - want).abs() <= 2.0 ** -8 * (v.float().abs().mean(1, keepdim=True) + want.abs()) + 1e-4)
+
+
+def test_blocks_of_rows_are_taken_longest_first():
+    import jax_flash_attn2 as J
+    B, S = 3, 2100
+    ids = ids_of([[(0, 2100)], [(0, 300), (1, 1000), (2, 500)], [(i, 100) for i in range(20)]], S)
+    order = J.document_layout(ids.cuda())[-B * 9:].tolist()
+    assert sorted(order) == list(range(B * 9))
+    seen = O.visible_keys(B, S, S, True, ids)
+
+    def length(i):
+        rows = seen[i // 9, i % 9 * 256:i % 9 * 256 + 256].any(0).nonzero().flatten()
+        return 0 if not len(rows) else rows[-1].item() // 128 - rows[0].item() // 128 + 1
+
+    lengths = [length(i) for i in order]
+    assert lengths == sorted(lengths, reverse=True)
+
+
 @pytest.mark.parametrize("cap", [2.0 ** -10, 0.5, 1024.0])
 def test_caps_at_the_ends_of_their_range(cap):
     # at 1024 the exponent's error is 2 * 1024 * log2(e) * 2^-23 = 3.5e-4, inside the slack of the bounds
