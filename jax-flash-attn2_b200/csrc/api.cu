@@ -592,13 +592,13 @@ int check_cache(const fa2_paged_cache& c, const char* what) {
 
 // 5-D map of 16-bit elements with a 128-byte swizzle.
 int encode_map(CUtensorMap* tm, const void* ptr, bool bf16, const cuuint64_t (&dims)[5], const cuuint64_t (&strides)[4],
-               const cuuint32_t (&box)[5], const char* what) {
+               const cuuint32_t (&box)[5], CUtensorMapL2promotion promotion, const char* what) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return fail(FA2_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                          const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(FA2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", what, static_cast<int>(r));
   return FA2_OK;
@@ -770,7 +770,7 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
                                 static_cast<cuuint64_t>(a->heads_kv)};
     const cuuint64_t st[4] = {bytes(a->q_stride_h), bytes(a->q_stride_t), bytes(hd.blk), bytes(a->q_stride_h * group)};
     const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tile_tokens), 1, 1};
-    if ((rc = encode_map(&L.tmQ, a->q, bf16, dims, st, box, "q"))) return rc;
+    if ((rc = encode_map(&L.tmQ, a->q, bf16, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, "q"))) return rc;
   }
   for (int x = 0; x < 2; ++x) {
     // (columns, places in a page, column blocks, heads, pages): a box is a piece of a page of at most 128 rows
@@ -780,7 +780,11 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
                                 static_cast<cuuint64_t>(a->pages)};
     const cuuint64_t st[4] = {bytes(c.stride_slot), bytes(hd.blk), bytes(c.stride_head), bytes(c.stride_page)};
     const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(std::min(a->page_size, 128)), 1, 1, 1};
-    if ((rc = encode_map(x ? &L.tmV : &L.tmK, c.ptr, bf16, dims, st, box, x ? "v_cache" : "k_cache"))) return rc;
+    // Up to 64 columns a key takes 128 bytes: fetching 256 would bring the next head's into L2, where it is not needed
+    // before another CTA comes there (16 decodes over 16000 keys, 16/8 heads, D = 64, pages of 64: 138 us, 121 with 128).
+    const CUtensorMapL2promotion promotion =
+        hd.padded == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+    if ((rc = encode_map(x ? &L.tmV : &L.tmK, c.ptr, bf16, dims, st, box, promotion, x ? "v_cache" : "k_cache"))) return rc;
   }
   PagedAttnDev& d = L.p;
   d.T = a->tokens; d.Hq = a->heads_q; d.Hkv = a->heads_kv; d.G = group;
