@@ -698,13 +698,43 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       uint32_t pg[has_cap(kMod) ? kCW / 2 : 1];
       const bool edge = kScored && (q_first < q_lo || q_first + kCW > q_hi);   // some of the queries do not see the key
       const float slope2 = has_slope(kMod) ? __ldg(p.mod.slopes + h) * kLog2e : 0.f;
-      {
+      if constexpr (has_cap(kMod)) {
+        // 32 queries at a time: their scores, P and P (1 - tanh^2) of all queries at once would not fit the registers
+        // (the packed P of a part goes over scores that have been read)
+#pragma unroll
+        for (int part = 0; part < kCW / 32; ++part) {
+          uint32_t s[32], pp[16];
+          tmem_ld32(tS + 32 * part, s);
+          tc_wait_ld();
+          tanh_row(reinterpret_cast<float(&)[32]>(s), p.mod.arg2);
+#pragma unroll
+          for (int c4 = 0; c4 < 8; ++c4) {
+            const float4 nl = nlse4[8 * part + c4];
+            const float nlv[4] = {nl.x, nl.y, nl.z, nl.w};
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+              const int c = 4 * c4 + 2 * k2, q = q_first + 32 * part + c;
+              float x0 = __uint_as_float(s[c]), x1 = __uint_as_float(s[c + 1]), g0, g1;
+              mod_exponents<kMod>(x0, x1, nlv[2 * k2], nlv[2 * k2 + 1], p.scale_log2, p.mod.cap2, slope2,
+                                  static_cast<float>(q_first + p.causal_off - kv) + static_cast<float>(32 * part + c), g0,
+                                  g1);
+              float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              if (edge) {
+                if (q < q_lo || q >= q_hi) p0 = 0.f;
+                if (q + 1 < q_lo || q + 1 >= q_hi) p1 = 0.f;
+              }
+              pg[16 * part + (c >> 1)] = pack2<kBf16>(p0 * g0, p1 * g1);
+              pp[c >> 1] = pack2<kBf16>(p0, p1);
+            }
+          }
+          tmem_st16(tS + 16 * part, pp);
+        }
+      } else {
         uint32_t s[kCW];
 #pragma unroll
         for (int c = 0; c < kCW / 32; ++c)
           tmem_ld32(tS + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
         tc_wait_ld();
-        if constexpr (has_cap(kMod)) tanh_row(reinterpret_cast<float(&)[kCW]>(s), p.mod.arg2);
         if constexpr (kFeat) {
 #pragma unroll
           for (int c = 0; c < kCW; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) * p.scale_log2);
@@ -760,7 +790,6 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 if (q_first + c < q_lo || q_first + c >= q_hi) p0 = 0.f;
                 if (q_first + c + 1 < q_lo || q_first + c + 1 >= q_hi) p1 = 0.f;
               }
-              if constexpr (has_cap(kMod)) pg[c >> 1] = pack2<kBf16>(p0 * g0, p1 * g1);
             } else if (diag) {
               if (q_first + c < q_lim) p0 = 0.f;
               if (q_first + c + 1 < q_lim) p1 = 0.f;
@@ -770,7 +799,9 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
       auto store_p = [&](const uint32_t (&x)[kCW / 2]) { tmem_st_cols(tS, x); };
-      if constexpr (kFeat) {
+      if constexpr (has_cap(kMod)) {
+        // stored already
+      } else if constexpr (kFeat) {
         if (p.drop.enabled) {
           // the weights that reach dV carry the dropout mask and its 1/(1-p)
           uint32_t pd[kCW / 2];
