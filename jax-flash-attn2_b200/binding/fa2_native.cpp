@@ -96,6 +96,11 @@ Tensor bytes_like(const Tensor& x, size_t n) {
   return at::empty({static_cast<int64_t>(n)}, x.options().dtype(at::kByte));
 }
 
+// Tells autograd of a write in place, so that a backward pass that saved `x` notices.
+void written(const Tensor& x) {
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- attention with changed scores -------------------------------------------------------------
 struct Scored {
   Tensor slopes, layout, prefix, rest;
@@ -286,7 +291,12 @@ PyObject* scored_flash_attention(PyObject*, PyObject* const* args, Py_ssize_t n)
   const size_t layout_bytes = ids.defined() || s.layout.defined()
                                   ? abi.document_layout_bytes(static_cast<int32_t>(batch), static_cast<int32_t>(sq))
                                   : 0;
-  if (s.layout.defined() && !vector_of(s.layout, at::kInt, static_cast<int64_t>(layout_bytes / 4), device)) Py_RETURN_NONE;
+  // [batch, words per row]: the shape tells the layout of one batch and length from that of another
+  const int64_t layout_words = static_cast<int64_t>(layout_bytes / 4) / batch;
+  if (s.layout.defined() &&
+      (s.layout.scalar_type() != at::kInt || s.layout.dim() != 2 || s.layout.size(0) != batch ||
+       s.layout.size(1) != layout_words || s.layout.device() != device || !s.layout.is_contiguous()))
+    Py_RETURN_NONE;
 
   const c10::cuda::CUDAGuard guard(device);
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
@@ -296,7 +306,7 @@ PyObject* scored_flash_attention(PyObject*, PyObject* const* args, Py_ssize_t n)
   {
     pybind11::gil_scoped_release no_gil;
     if (ids.defined()) {
-      s.layout = at::empty({static_cast<int64_t>(layout_bytes / 4)}, q.options().dtype(at::kInt));
+      s.layout = at::empty({batch, layout_words}, q.options().dtype(at::kInt));
       refused = abi.document_layout(ids.const_data_ptr<int32_t>(), ids.stride(0), static_cast<int32_t>(batch),
                                     static_cast<int32_t>(sq), s.layout.data_ptr<int32_t>(), layout_bytes,
                                     stream_of(q)) != FA2_OK;
@@ -340,10 +350,10 @@ PyObject* paged_step_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !vector_of(fresh, at::kInt, requests, device) || free.dim() != 1 || !vector_of(free, at::kInt, free.size(0), device))
     Py_RETURN_NONE;
   if (start.defined() && !vector_of(start, at::kInt, 1, device)) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(device);
   const size_t bytes = abi.paged_work_bytes(static_cast<int32_t>(requests), static_cast<int32_t>(tokens),
                                             static_cast<int32_t>(heads_q), static_cast<int32_t>(heads_kv));
   if (bytes == 0) Py_RETURN_NONE;
-  const c10::cuda::CUDAGuard guard(device);
   const int64_t ints = static_cast<int64_t>(bytes / 4);
   const auto options = table.options();
   const Tensor work = at::empty({ints}, options), cu = at::empty({requests + 1}, options), lens = at::empty({requests}, options),
@@ -371,6 +381,7 @@ PyObject* paged_step_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.work = work.data_ptr<int32_t>();
   a.work_bytes = bytes;
   if (abi.paged_plan(&a, stream_of(table)) != FA2_OK) Py_RETURN_NONE;
+  written(table);
   PyObject* result = PyTuple_New(6);
   if (!result) return nullptr;
   const Tensor* parts[6] = {&cu, &lens, &slots, &positions, &taken, &work};
@@ -398,6 +409,8 @@ PyObject* paged_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
       v.device() != kc.device() || k.stride(2) != 1 || v.stride(2) != 1 || k.size(0) > INT32_MAX ||
       !vector_of(slots, at::kLong, k.size(0), kc.device()))
     Py_RETURN_NONE;
+  if (at::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad() || kc.requires_grad() || vc.requires_grad()))
+    Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(kc.device());
   fa2_paged_write_params a = {};
   a.k = k.const_data_ptr(); a.k_stride_t = k.stride(0); a.k_stride_h = k.stride(1);
@@ -411,6 +424,8 @@ PyObject* paged_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.pages = static_cast<int32_t>(kc.size(0));
   a.page_size = static_cast<int32_t>(kc.size(1));
   if (abi.paged_cache_write(&a, stream_of(kc)) != FA2_OK) Py_RETURN_NONE;
+  written(kc);
+  written(vc);
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -431,12 +446,17 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (!caches_ok(kc, vc) || q.dim() != 3 || q.size(0) != tokens || q.size(1) != heads_q || q.size(2) != kc.size(3) ||
       kc.size(2) != heads_kv || kc.size(1) != page || q.scalar_type() != kc.scalar_type() || q.device() != kc.device() ||
-      work.device() != kc.device() || q.stride(2) != 1)
+      work.device() != kc.device() || work.scalar_type() != at::kInt || q.stride(2) != 1)
+    Py_RETURN_NONE;
+  if (table.device() != kc.device() || table.scalar_type() != at::kInt || table.dim() != 2 || table.numel() == 0 ||
+      table.stride(1) != 1)
     Py_RETURN_NONE;
   if (!optional_number(args[9], 1.0 / std::sqrt(static_cast<double>(kc.size(3))), &scale) ||
       !optional_number(args[10], 0.0, &cap) || !softcap_ok(cap))
     Py_RETURN_NONE;
-  if (at::GradMode::is_enabled() && (q.requires_grad() || kc.requires_grad() || vc.requires_grad())) Py_RETURN_NONE;
+  if (at::GradMode::is_enabled() && (q.requires_grad() || kc.requires_grad() || vc.requires_grad() ||
+                                     (out.defined() && out.requires_grad()) || (lse.defined() && lse.requires_grad())))
+    Py_RETURN_NONE;
   if (slopes.defined() && (!vector_of(slopes, at::kFloat, heads_q, q.device()) || slopes.requires_grad())) Py_RETURN_NONE;
   if (lse.defined() && (lse.scalar_type() != at::kFloat || lse.dim() != 2 || lse.size(0) != tokens || lse.size(1) != heads_q ||
                         lse.device() != q.device() || !lse.is_contiguous()))
@@ -473,6 +493,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.workspace = workspace.data_ptr();
   a.workspace_bytes = bytes;
   if (abi.paged_attention(&a, stream_of(q)) != FA2_OK) Py_RETURN_NONE;
+  written(out);
+  if (lse.defined()) written(lse);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }

@@ -105,7 +105,9 @@ def paged_step_plan(
     if free_start is not None:
         free_start = _check_int32(free_start.reshape(-1), (1,), "free_start", device)
     lib = _capi.load()
-    nbytes = lib.fa2_paged_work_bytes(requests, num_tokens, heads_q, heads_kv)
+    heads_q, heads_kv = int(heads_q), int(heads_kv)
+    with torch.cuda.device(device):
+        nbytes = lib.fa2_paged_work_bytes(requests, num_tokens, heads_q, heads_kv)
     if nbytes == 0:
         _capi.check(_capi.FA2_ERR_INVALID_ARG)
     # one buffer for all int32 results: work list (16-byte aligned), row starts, lengths, positions, pages taken
@@ -124,8 +126,20 @@ def paged_step_plan(
     a.positions, a.pages_taken = positions.data_ptr(), pages_taken.data_ptr()
     a.work, a.work_bytes = work.data_ptr(), nbytes
     _launch(lib.fa2_paged_plan, a, device)
+    _written(block_table)
     return PagedStepPlan(cu_seqlens, seqlens_k, block_table, slot_map, positions, pages_taken, work, page_size, num_tokens,
                          heads_q, heads_kv)
+
+
+def _written(x: torch.Tensor) -> None:
+    """Tells autograd of a write in place, so that a backward pass that saved `x` notices."""
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+
+
+def _check_no_grad(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
 
 
 def _cache(x: torch.Tensor, name: str) -> _capi.PagedCache:
@@ -147,12 +161,14 @@ def _check_caches(k_cache, v_cache):
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       slot_map: torch.Tensor) -> None:
     """Writes row t of k and v ([T, Hkv, D], strided rows and heads allowed) to slot `slot_map[t]` (int64 [T]) of the
-    caches [pages, page_size, Hkv, D]. Slots outside the cache (-1) are skipped; no slot may occur twice."""
+    caches [pages, page_size, Hkv, D]. Slots outside the cache (-1) are skipped; no slot may occur twice. No gradients:
+    inference only."""
     if _native.load().paged_cache_write(k, v, k_cache, v_cache, slot_map):
         return
     # the call is to be refused, or some operand has to be copied first
     if not k_cache.is_cuda:
         raise RuntimeError("fa2_b200 runs on CUDA tensors only; there is no CPU path")
+    _check_no_grad("paged_cache_write", k, v, k_cache, v_cache)
     _check_caches(k_cache, v_cache)
     a = _capi.PagedWriteParams()
     a.k_cache, a.v_cache = _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache")
@@ -176,6 +192,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     a.slot_map = slot_map.data_ptr()
     a.tokens, a.heads, a.head_dim, a.pages, a.page_size = tokens, heads, d, pages, page_size
     _launch(_capi.load().fa2_paged_cache_write, a, k_cache.device)
+    _written(k_cache)
+    _written(v_cache)
 
 
 def paged_attention(
@@ -205,8 +223,7 @@ def paged_attention(
     # the call is to be refused, or some operand has to be copied first
     if not q.is_cuda:
         raise RuntimeError("fa2_b200 runs on CUDA tensors only; there is no CPU path")
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
-        raise RuntimeError("paged_attention has no backward pass: call it under torch.no_grad()")
+    _check_no_grad("paged_attention", q, k_cache, v_cache, out, lse)
     _check_caches(k_cache, v_cache)
     a = _capi.PagedAttentionParams()
     a.k_cache, a.v_cache = _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache")
@@ -217,8 +234,11 @@ def paged_attention(
     if (tokens, heads_q, heads_kv, page_size) != (plan.num_tokens, plan.heads_q, plan.heads_kv, plan.page_size):
         raise ValueError(f"the plan is for {plan.num_tokens} tokens, {plan.heads_q} / {plan.heads_kv} heads and pages of "
                          f"{plan.page_size}, got {tokens} tokens, {heads_q} / {heads_kv} heads and pages of {page_size}")
-    if not (q.device == k_cache.device == plan.work.device):
+    table = plan.block_table
+    if not (q.device == k_cache.device == plan.work.device == table.device):
         raise ValueError("q, the caches and the plan must live on one device")
+    if plan.work.dtype != torch.int32 or table.dtype != torch.int32 or table.dim() != 2 or 0 in table.shape or table.stride(1) != 1:
+        raise ValueError("the plan must be what paged_step_plan returned")
     if q.stride(2) != 1:
         q = q.contiguous()
     if out is None:
@@ -235,7 +255,6 @@ def paged_attention(
     a.o, a.o_stride_t, a.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
     a.tokens, a.heads_q, a.heads_kv, a.head_dim, a.dtype = tokens, heads_q, heads_kv, d, _DTYPE_CODE[q.dtype]
     a.pages, a.page_size = pages, page_size
-    table = plan.block_table
     a.block_table, a.table_width, a.requests = table.data_ptr(), table.shape[1], table.shape[0]
     a.table_stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
     a.work = plan.work.data_ptr()
@@ -248,4 +267,7 @@ def paged_attention(
     workspace = torch.empty((max(nbytes, 128),), dtype=torch.uint8, device=q.device)
     a.workspace, a.workspace_bytes = workspace.data_ptr(), nbytes
     _launch(lib.fa2_paged_attention, a, q.device)
+    _written(out)
+    if lse is not None:
+        _written(lse)
     return out

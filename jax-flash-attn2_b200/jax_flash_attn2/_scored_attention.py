@@ -61,7 +61,8 @@ def document_layout(document_ids: torch.Tensor) -> torch.Tensor:
     nbytes = lib.fa2_document_layout_bytes(batch, seqlen)
     if nbytes == 0:
         raise ValueError("document_ids must not be empty")
-    layout = torch.empty((nbytes // 4,), dtype=torch.int32, device=document_ids.device)
+    # (the shape tells the layout of one batch and length from that of another)
+    layout = torch.empty((batch, nbytes // 4 // batch), dtype=torch.int32, device=document_ids.device)
     index = document_ids.device.index
     with torch.cuda.device(index):
         stream = torch.cuda.current_stream(index).cuda_stream
@@ -95,8 +96,8 @@ def _score_mod(q, k, causal, softcap, alibi_slopes, layout, prefix_lens, rest=No
     if layout is not None:
         if k.shape[1] != sq:
             raise ValueError("documents need as many keys as queries")
-        need = batch * (2 * sq + 2 * ((sq + 127) // 128) + (sq + 255) // 256)
-        if layout.dtype != torch.int32 or layout.numel() != need or not layout.is_contiguous() or layout.device != q.device:
+        words = _capi.load().fa2_document_layout_bytes(batch, sq) // 4 // batch
+        if layout.dtype != torch.int32 or tuple(layout.shape) != (batch, words) or not layout.is_contiguous() or layout.device != q.device:
             raise ValueError("layout must be what document_layout returned for ids of shape "
                              f"[{batch}, {sq}] on the device of q")
         mod.document_layout = layout.data_ptr()

@@ -269,3 +269,31 @@ def test_paged_python_layer_refuses_before_any_launch():
         J._paged._check_caches(cache, cache[:2])
     with pytest.raises(ValueError, match="fp16 or bf16"):
         J._paged._check_caches(cache.float(), cache.float())
+
+
+def test_a_layout_serves_the_shape_it_was_made_for_alone():
+    # [1, 512] and [2, 256] take the same number of words: the shape tells them apart
+    words = lambda b, s: J._capi.load().fa2_document_layout_bytes(b, s) // 4
+    assert words(1, 512) == words(2, 256)
+    short, long = torch.zeros(2, 256, 1, 64, dtype=torch.bfloat16), torch.zeros(1, 512, 1, 64, dtype=torch.bfloat16)
+    layout = torch.zeros(1, words(1, 512), dtype=torch.int32)
+    mods = J._scored_attention._score_mod
+    mods(long, long, True, None, None, layout, None)
+    for wrong in (layout.view(2, -1), layout.view(-1), layout[:, :-1]):
+        with pytest.raises(ValueError, match="document_layout"):
+            mods(long, long, True, None, None, wrong, None)
+    with pytest.raises(ValueError, match="document_layout"):
+        mods(short, short, True, None, None, layout, None)
+
+
+def test_serving_calls_take_no_part_in_training():
+    x = torch.zeros(2, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        J._paged._check_no_grad("paged_cache_write", torch.zeros(2), None, x)
+    with torch.no_grad():
+        J._paged._check_no_grad("paged_cache_write", x)
+    y = torch.zeros(2)
+    J._paged._written(y)
+    assert y._version == 1
+    with torch.inference_mode():
+        J._paged._written(torch.zeros(2))

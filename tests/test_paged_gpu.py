@@ -390,3 +390,32 @@ def test_calls_that_are_not_offered():
         J.paged_attention(torch.zeros(1, 4, 256, dtype=BF16, device="cuda"), wide, wide, plan)
     with pytest.raises(ValueError, match="slot_map"):
         J.paged_cache_write(cache[0, :1], cache[0, :1], cache, cache, torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+def test_writes_in_place_are_known_to_autograd():
+    import jax_flash_attn2 as J
+    cache, other = (torch.zeros(4, 16, 2, 64, dtype=BF16, device="cuda") for _ in range(2))
+    table = dev_int([[0]])
+    plan = J.paged_step_plan(dev_int([5]), dev_int([1]), table, dev_int([1]), page_size=16, num_tokens=1, heads_q=4, heads_kv=2)
+    k = torch.ones(1, 2, 64, dtype=BF16, device="cuda")
+    J.paged_cache_write(k, k, cache, other, plan.slot_map)
+    out, lse = torch.zeros(1, 4, 64, dtype=BF16, device="cuda"), torch.zeros(1, 4, device="cuda")
+    J.paged_attention(out.clone(), cache, other, plan, out=out, lse=lse)
+    assert [x._version for x in (table, cache, other, out, lse)] == [1] * 5
+    # copied operands go through the Python function
+    J.paged_cache_write(k.transpose(1, 2).contiguous().transpose(1, 2), k, cache, other, plan.slot_map)
+    assert cache._version == 2 and other._version == 2
+    with pytest.raises(RuntimeError, match="no backward"):
+        J.paged_cache_write(k.clone().requires_grad_(True), k, cache, other, plan.slot_map)
+    with pytest.raises(RuntimeError, match="no backward"):
+        J.paged_attention(out.detach(), cache, other, plan, out=torch.zeros_like(out).requires_grad_(True))
+    with torch.inference_mode():
+        fresh = torch.zeros(4, 16, 2, 64, dtype=BF16, device="cuda")
+        J.paged_cache_write(k, k, fresh, fresh.clone(), plan.slot_map)
+    assert torch.equal(fresh, cache)
+    plan.block_table = table.cpu()
+    with pytest.raises(ValueError, match="one device"):
+        J.paged_attention(out.detach(), cache, other, plan)
+    plan.block_table = table.long()
+    with pytest.raises(ValueError, match="paged_step_plan"):
+        J.paged_attention(out.detach(), cache, other, plan)
