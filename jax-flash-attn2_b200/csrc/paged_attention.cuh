@@ -59,11 +59,15 @@ struct PagedSmem {
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
 };
 
-// A CTA's way from its start to the next CTA's.
+// A CTA's way from its start to the next CTA's. An item it begins inside of comes last, so that the CTAs, which all begin with
+// the first key tile of some item, walk over the keys of a long request side by side and share them in L2: 4096 new tokens of
+// 64/8 heads, D = 128, over 65536 keys 8.55 -> 7.77 ms, over 32768 3.75 -> 3.67, over 8192 (which fit L2 either way)
+// 0.678 -> 0.690.
 struct PagedWalk {
   int n_items;
   int hk, i, tile;
   int end_hk, end_i, end_tile;
+  int late;                     // the stretch at the CTA's start is still to come
 };
 
 // One stretch of it: key tiles [ja, jb) of one item and head.
@@ -90,37 +94,55 @@ __device__ __forceinline__ int4 paged_start_of(const int* work, int c) {
   return __ldg(reinterpret_cast<const int4*>(work + kWorkHeader) + c);
 }
 
+__device__ __forceinline__ void paged_advance(PagedWalk& w) {
+  if (++w.i == w.n_items) {
+    w.i = 0;
+    ++w.hk;
+  }
+}
+
 __device__ __forceinline__ void paged_start(const PagedAttnDev& p, PagedWalk& w) {
   w.n_items = __ldg(p.work);
   const int ctas = __ldg(p.work + 1), c = blockIdx.x;
-  w.hk = w.i = w.tile = w.end_hk = w.end_i = w.end_tile = 0;
+  w.hk = w.i = w.tile = w.end_hk = w.end_i = w.end_tile = w.late = 0;
   if (c >= ctas) return;
   const int4 from = paged_start_of(p.work, c), to = paged_start_of(p.work, c + 1);
   w.hk = from.x; w.i = from.y; w.tile = from.z;
   w.end_hk = to.x; w.end_i = to.y; w.end_tile = to.z;
+  if (w.tile > 0 && (w.hk != w.end_hk || w.i != w.end_i)) {
+    w.late = 1;
+    w.tile = 0;
+    paged_advance(w);
+  }
 }
 
 __device__ __forceinline__ bool paged_next(const PagedAttnDev& p, PagedWalk& w, PagedSeg& s) {
-  const bool in_last = w.hk == w.end_hk && w.i == w.end_i;
-  if (in_last && w.tile >= w.end_tile) return false;
-  const int4* item = reinterpret_cast<const int4*>(p.work + p.items_at) + 2 * static_cast<long long>(w.i);
+  bool in_last = w.hk == w.end_hk && w.i == w.end_i;
+  int4 at = make_int4(w.hk, w.i, w.tile, 0);
+  const bool done = in_last && w.tile >= w.end_tile;
+  if (done) {
+    if (!w.late) return false;
+    w.late = 0;
+    in_last = false;
+    at = paged_start_of(p.work, blockIdx.x);
+  }
+  const int4* item = reinterpret_cast<const int4*>(p.work + p.items_at) + 2 * static_cast<long long>(at.y);
   const int4 a = __ldg(item);
   s.tiles = __ldg(&item[1].y);
-  s.hk = w.hk;
+  s.hk = at.x;
   s.row0 = a.x;
   s.n_tok = a.y;
   s.pos0 = a.z;
   s.req = a.w;
-  s.ja = w.tile;
+  s.ja = at.z;
   s.jb = in_last ? w.end_tile : s.tiles;
   s.seen = min(s.pos0 + s.n_tok, p.table_width << p.page_shift);
   s.whole = s.ja == 0 && s.jb == s.tiles;
-  w.tile = s.jb;
-  if (s.jb == s.tiles) {
-    w.tile = 0;
-    if (++w.i == w.n_items) {
-      w.i = 0;
-      ++w.hk;
+  if (!done) {
+    w.tile = s.jb;
+    if (s.jb == s.tiles) {
+      w.tile = 0;
+      paged_advance(w);
     }
   }
   s.dual = s.n_tok <= p.tile_tokens;
@@ -407,6 +429,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       note->w.n_items = w.n_items;
       note->w.hk = w.hk; note->w.i = w.i; note->w.tile = w.tile;
       note->w.end_hk = w.end_hk; note->w.end_i = w.end_i; note->w.end_tile = w.end_tile;
+      note->w.late = w.late;
     }
     __syncwarp();
     while (true) {
@@ -417,6 +440,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         w.n_items = note->w.n_items;
         w.hk = note->w.hk; w.i = note->w.i; w.tile = note->w.tile;
         w.end_hk = note->w.end_hk; w.end_i = note->w.end_i; w.end_tile = note->w.end_tile;
+        w.late = note->w.late;
         PagedSeg s;
         if (!paged_next(p, w, s)) break;
         const int tok = r / p.G, head = r - tok * p.G;     // this row's token in the tile and head in the group
@@ -433,6 +457,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         __syncwarp();
         if (lane == 0) {
           note->w.hk = w.hk; note->w.i = w.i; note->w.tile = w.tile;
+          note->w.late = w.late;
           note->row0 = s.row0 + tok0;
           note->hk = s.hk;
           // the first stretch of a CTA that begins inside an item, the last one that ends inside one
