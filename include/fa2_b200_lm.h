@@ -17,7 +17,7 @@ extern "C" {
 #endif
 
 /* Version of this header (major * 1000 + minor), apart from that of fa2_b200.h. */
-#define FA2_LM_ABI_VERSION 1000
+#define FA2_LM_ABI_VERSION 1001
 int fa2_lm_version(void);
 
 /* ---------------------------------------------------------------------------------------------
@@ -54,8 +54,12 @@ int fa2_document_layout(const int32_t* document_ids, int64_t stride_b, int32_t b
 
 /* fa2_fwd / fa2_bwd with changed scores. The parameter blocks are those of fa2_b200.h without bias,
  * mask, dropout, seqlens, dbias and dropout_bits (refused); softmax_scale must be positive;
- * fa2_fwd_workspace_bytes / fa2_bwd_workspace_bytes size the scratch. */
+ * fa2_fwd_workspace_bytes sizes the scratch of the forward. The backward needs fa2_bwd_workspace_bytes; with
+ * fa2_scored_bwd_workspace_bytes it may deal the query heads of a key/value head to several SMs where there are few tiles
+ * (dk and dv are the same from call to call either way, but not between the two). Both depend on the current device's
+ * number of SMs. */
 int fa2_scored_fwd(const fa2_fwd_params* params, const fa2_score_mod* mod, void* cuda_stream);
+size_t fa2_scored_bwd_workspace_bytes(const fa2_problem* problem);
 int fa2_scored_bwd(const fa2_bwd_params* params, const fa2_score_mod* mod, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -36,7 +36,7 @@ struct Abi {
   decltype(&fa2_document_layout_bytes) document_layout_bytes;
   decltype(&fa2_document_layout) document_layout;
   decltype(&fa2_fwd_workspace_bytes) fwd_workspace_bytes;
-  decltype(&fa2_bwd_workspace_bytes) bwd_workspace_bytes;
+  decltype(&fa2_scored_bwd_workspace_bytes) scored_bwd_workspace_bytes;
   decltype(&fa2_scored_fwd) scored_fwd;
   decltype(&fa2_scored_bwd) scored_bwd;
   decltype(&fa2_paged_work_bytes) paged_work_bytes;
@@ -200,7 +200,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     const Tensor d_o = laid_out(grads[0]);
     fa2_bwd_params a = {};
     a.p = problem_of(q, k, s);
-    const size_t n = abi.bwd_workspace_bytes(&a.p);
+    const size_t n = abi.scored_bwd_workspace_bytes(&a.p);
     const Tensor workspace = bytes_like(q, n);
     for (int i = 0; i < 3; ++i) result[i] = at::empty(saved[i].sizes(), q.options());
     a.q = q.const_data_ptr(); a.q_strides = strides_of(q);

@@ -269,7 +269,25 @@ size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 struct BwdWorkspace {
   size_t delta_off, dq_off, absmax_off, xstats_off, order_off, total;
   int sq_pad;
+  // attention with changed scores: the parts of the query heads and their dK and dV behind all else
+  int parts;
+  size_t parts_off, parts_total;
 };
+// Parts into which the backward of attention with changed scores deals the query heads of a key/value head: as many (a
+// divisor of them) as find an SM each, if that takes at least 2 of the 128-query steps off a key tile's way; joining the parts
+// costs about as much as one step, 2 to 3 us. Measured (causal, bf16, whole backward, one part -> parts): 4096 queries, 16/2
+// heads, D = 128 633 -> 346 us, 16/1 heads, D = 64 915 -> 251 us; 1 x 512, 32/8 heads, D = 128 63 -> 40 us; 1 x 1024, 8/1 heads,
+// D = 256 256 -> 64 us; two steps less: 1 x 256, 8/4 heads, D = 128 33 -> 31 us; one less: 1 x 128, 8/4 heads, D = 128 28 -> 33 us
+// (with a join of twice today's time).
+int bwd_parts(const fa2_problem& p, const HeadDim& hd) {
+  const int64_t tiles = static_cast<int64_t>(p.batch) * p.heads_kv * ((p.seqlen_k + 127) / 128) * (hd.padded == 256 ? 2 : 1);
+  const int64_t group = p.heads_q / p.heads_kv, room = sm_count() / tiles;
+  int64_t parts = 1;
+  for (int64_t d = 2; d <= std::min(group, room); ++d)
+    if (group % d == 0) parts = d;
+  const int64_t steps = (static_cast<int64_t>(p.seqlen_q) + 127) / 128 * group;
+  return steps - steps / parts >= 2 ? static_cast<int>(parts) : 1;
+}
 BwdWorkspace bwd_workspace(const fa2_problem& p) {
   BwdWorkspace w;
   w.sq_pad = (p.seqlen_q + 127) / 128 * 128;
@@ -286,6 +304,10 @@ BwdWorkspace bwd_workspace(const fa2_problem& p) {
   // counters for the bit-reproducible mode: one per 128-row dQ tile, at head dim 256 one per
   // 64 rows and half of the head dim
   w.total = w.order_off + align_up(rows / 128 * (hd.padded <= 128 ? 1 : 4) * sizeof(int), 256);
+  w.parts = bwd_parts(p, hd);
+  w.parts_off = w.total;
+  const size_t kv_rows = static_cast<size_t>(p.batch) * p.heads_kv * ((static_cast<size_t>(p.seqlen_k) + 127) / 128 * 128);
+  w.parts_total = w.total + (w.parts > 1 ? 2 * w.parts * kv_rows * hd.padded * sizeof(float) : 0);
   return w;
 }
 
@@ -523,6 +545,11 @@ int fa2_lm_version(void) { return FA2_LM_ABI_VERSION; }
 int fa2_scored_fwd(const fa2_fwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
   if (!mod) return fail(FA2_ERR_INVALID_ARG, "mod is null");
   return fwd_impl(a, mod, cuda_stream);
+}
+
+size_t fa2_scored_bwd_workspace_bytes(const fa2_problem* problem) {
+  if (!problem || check_problem(*problem)) return 0;
+  return bwd_workspace(*problem).parts_total;
 }
 
 int fa2_scored_bwd(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
@@ -1091,6 +1118,13 @@ int bwd_impl(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_strea
   L.o = a->o; L.o_strides[0] = a->o_strides.b; L.o_strides[1] = a->o_strides.s; L.o_strides[2] = a->o_strides.h;
   L.d_o = a->d_o; L.do_strides[0] = a->do_strides.b; L.do_strides[1] = a->do_strides.s; L.do_strides[2] = a->do_strides.h;
   L.dq = a->dq; L.dq_strides[0] = a->dq_strides.b; L.dq_strides[1] = a->dq_strides.s; L.dq_strides[2] = a->dq_strides.h;
+  L.parts = 1;
+  if (mod && w.parts > 1 && a->workspace_bytes >= w.parts_total) {
+    L.parts = w.parts;
+    kp.part_kv = reinterpret_cast<float*>(ws + w.parts_off);
+    L.dk = a->dk; L.dk_strides[0] = a->dk_strides.b; L.dk_strides[1] = a->dk_strides.s; L.dk_strides[2] = a->dk_strides.h;
+    L.dv = a->dv; L.dv_strides[0] = a->dv_strides.b; L.dv_strides[1] = a->dv_strides.s; L.dv_strides[2] = a->dv_strides.h;
+  }
   L.delta = reinterpret_cast<float*>(ws + w.delta_off);
   L.dq_acc_bytes = w.absmax_off - w.dq_off;
   L.head_dim_real = p.head_dim;

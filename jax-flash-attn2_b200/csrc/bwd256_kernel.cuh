@@ -100,7 +100,7 @@ bwd256_dq_convert(const float* __restrict__ dq_acc, uint16_t* __restrict__ dq, l
   }
 }
 
-template <bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod>
+template <bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod, bool kParts = false>
 __global__ void __launch_bounds__(kThreads256, 1)
 bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -161,7 +161,9 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   int i_end = nQ64_b;
   if constexpr (kScored) key_tile_range<kBQ>(p.mod, b, n, p.Sq, p.causal_off, i_start, i_end);
   const int nI = i_end - i_start;
-  const int T = (n * kBK < sk_b) ? nI * p.G : 0;    // steps of this CTA (none: dK = dV = 0)
+  const int heads = kParts ? p.G / static_cast<int>(gridDim.y) : p.G;      // query heads of this CTA
+  const int h0 = hk * p.G + (kParts ? static_cast<int>(blockIdx.y) * heads : 0);
+  const int T = (n * kBK < sk_b) ? nI * heads : 0;  // steps of this CTA (none: dK = dV = 0)
   const bool dead_keys = n * kBK + kBK > sk_b;      // some key rows lie past the end
 
   if (tid == 0) {
@@ -204,7 +206,7 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   auto step_coords = [&](int it, int& h, int& i) {
     const int g = it / nI;
     i = i_start + (it - g * nI);
-    h = hk * p.G + g;
+    h = h0 + g;
   };
 
   if (warp >= 12) setmaxnreg_dec<kRegsOther256>();
@@ -642,6 +644,10 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
           for (int k = 0; k < 32; ++k) a[k] = 0u;
         }
+        if constexpr (kParts) {
+          store_part_columns(part_tile<kD>(p, w, bhk, n), half * 32 + c * 8, r, a, f);
+          continue;
+        }
         uint8_t* line = stage + (c >> 1) * L::kKBlock + r * 128;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
@@ -657,7 +663,7 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       fence_proxy_async_smem();
     }
     named_bar_sync(1 + w, 128);
-    if (ok && r == 0 && !*abort_flag) {
+    if (ok && r == 0 && !*abort_flag && !kParts) {
       tma_store_5d(w == 0 ? &tmdK : &tmdV, w == 0 ? sQ : sdO, 0, n * kBK, 2 * half, hk, b);
       tma_store_commit();
       tma_store_wait_read0();
@@ -673,15 +679,15 @@ bwd256_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   }
 }
 
-template <bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod>
+template <bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod, bool kParts = false>
 static cudaError_t launch256_main(const BwdLaunch& a, cudaStream_t stream) {
   using L = BSmem256;
-  auto kern = bwd256_main_kernel<kBf16, kCausal, kFeat, kMod>;
+  auto kern = bwd256_main_kernel<kBf16, kCausal, kFeat, kMod, kParts>;
   static bool smem_opted_in[64] = {};
   cudaError_t e = opt_in_dynamic_smem(kern, L::kDynamicBytes, smem_opted_in);
   if (e != cudaSuccess) return e;
   const long long nblocks = 2LL * a.kp.n_kvblk * a.kp.B * a.kp.Hkv;
-  kern<<<static_cast<unsigned>(nblocks), kThreads256, L::kDynamicBytes, stream>>>(
+  kern<<<dim3(static_cast<unsigned>(nblocks), a.parts), kThreads256, L::kDynamicBytes, stream>>>(
       a.tmQ, a.tmK, a.tmV, a.tmdO, a.tmdK, a.tmdV, a.delta, a.kp);
   return cudaGetLastError();
 }
@@ -715,6 +721,7 @@ static cudaError_t launch256_passes(const BwdLaunch& a, cudaStream_t stream, Mai
   bwd256_dq_convert<kBf16><<<static_cast<unsigned>(static_cast<long long>(nQ64) * kp.B * kp.Hq), 256, 0, stream>>>(
       kp.dq_acc, static_cast<uint16_t*>(a.dq), a.dq_strides[0], a.dq_strides[1], a.dq_strides[2],
       kp.Sq, kp.Hq, nQ64, kp.scale, kBf16 ? nullptr : kp.do_absmax_bits, a.head_blk);
+  if (kp.part_kv != nullptr) launch_kv_join<kD, kBf16>(a, stream);
   mark(3);
   return cudaGetLastError();
 }

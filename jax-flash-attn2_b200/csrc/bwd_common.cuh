@@ -2,6 +2,7 @@
 // scale, score-term loads and the pre-pass kernel.
 #pragma once
 #include <cuda_bf16.h>
+#include "bwd_launch.cuh"
 #include "kernel_params.cuh"
 #include "ptx_sm100.cuh"
 
@@ -286,5 +287,82 @@ bwd_pre_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ d_o,
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Query heads of a key/value head dealt to several CTAs (BwdKernelParams::part_kv)
+// ---------------------------------------------------------------------------------------------
+// The tile of this CTA's part of dK (acc = 0) or dV (1).
+template <int D>
+__device__ __forceinline__ float4* part_tile(const BwdKernelParams& p, int acc, int bhk, int n) {
+  const long long tiles = static_cast<long long>(p.B) * p.Hkv * p.n_kvblk;
+  return reinterpret_cast<float4*>(p.part_kv) +
+         ((2LL * blockIdx.y + acc) * tiles + static_cast<long long>(bhk) * p.n_kvblk + n) * (D / 4 * 128);
+}
+// 32 columns of key row `r`, from column 4 * chunk on, times f.
+__device__ __forceinline__ void store_part_columns(float4* tile, int chunk, int r, const uint32_t (&a)[32], float f) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    tile[(chunk + k) * 128 + r] = make_float4(__uint_as_float(a[4 * k]) * f, __uint_as_float(a[4 * k + 1]) * f,
+                                              __uint_as_float(a[4 * k + 2]) * f, __uint_as_float(a[4 * k + 3]) * f);
+}
+
+// dK and dV from their parts, added in the order of the heads and rounded once. A block takes 64 columns of 32 keys: the parts
+// are read along the keys, and turned through shared memory to be written along the columns. There is little of it (it runs
+// where a key tile per SM at most is computed), so blocks are small and each thread's loads are under way together.
+struct KvJoin {
+  const float4* parts;
+  int n_parts, n_kvblk, Hkv, Sk, blk_real;
+  long long tiles;                       // of dK in one part
+  uint16_t* out[2];                      // dK, dV
+  long long sb[2], ss[2], sh[2];
+};
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256)
+bwd_kv_join_kernel(const KvJoin p) {
+  constexpr int kPitch = 33;             // float4 per column chunk: 32 keys and one of padding
+  __shared__ float4 tile[16 * kPitch];
+  const int key0 = blockIdx.x % 4 * 32, blk = blockIdx.x / 4 % (D / 64), acc = blockIdx.y;
+  const long long t = blockIdx.x / (4 * (D / 64));
+  const int n = static_cast<int>(t % p.n_kvblk);
+  const long long bhk = t / p.n_kvblk;
+  const int b = static_cast<int>(bhk / p.Hkv), hk = static_cast<int>(bhk - static_cast<long long>(b) * p.Hkv);
+  const int tid = threadIdx.x;
+  float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  const float4* src = p.parts + (acc * p.tiles + t) * (D / 4 * 128) + blk * 2048 + key0 + (tid >> 5) * 128 + (tid & 31);
+#pragma unroll 4
+  for (int y = 0; y < p.n_parts; ++y, src += 2 * p.tiles * (D / 4 * 128)) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {        // column chunks tid / 32 and 8 further on
+      const float4 v = __ldcg(src + k * 1024);
+      sum[k].x += v.x; sum[k].y += v.y; sum[k].z += v.z; sum[k].w += v.w;
+    }
+  }
+  tile[(tid >> 5) * kPitch + (tid & 31)] = sum[0];
+  tile[(8 + (tid >> 5)) * kPitch + (tid & 31)] = sum[1];
+  __syncthreads();
+  const int j = tid & 7, r = tid >> 3;
+  const long long row = static_cast<long long>(n) * 128 + key0 + r;
+  if (row >= p.Sk || 8 * j >= p.blk_real) return;
+  const float4 x = tile[(2 * j) * kPitch + r], y = tile[(2 * j + 1) * kPitch + r];
+  reinterpret_cast<uint4*>(p.out[acc] + b * p.sb[acc] + row * p.ss[acc] + hk * p.sh[acc])[blk * (p.blk_real >> 3) + j] =
+      make_uint4(pack2<kBf16>(x.x, x.y), pack2<kBf16>(x.z, x.w), pack2<kBf16>(y.x, y.y), pack2<kBf16>(y.z, y.w));
+}
+template <int D, bool kBf16>
+static void launch_kv_join(const BwdLaunch& a, cudaStream_t stream) {
+  KvJoin j;
+  j.parts = reinterpret_cast<const float4*>(a.kp.part_kv);
+  j.n_parts = a.parts;
+  j.n_kvblk = a.kp.n_kvblk;
+  j.Hkv = a.kp.Hkv;
+  j.Sk = a.kp.Sk;
+  j.blk_real = a.head_blk;
+  j.tiles = static_cast<long long>(a.kp.B) * a.kp.Hkv * a.kp.n_kvblk;
+  j.out[0] = static_cast<uint16_t*>(a.dk);
+  j.out[1] = static_cast<uint16_t*>(a.dv);
+  for (int x = 0; x < 2; ++x) {
+    const long long* st = x ? a.dv_strides : a.dk_strides;
+    j.sb[x] = st[0]; j.ss[x] = st[1]; j.sh[x] = st[2];
+  }
+  bwd_kv_join_kernel<D, kBf16><<<dim3(static_cast<unsigned>(j.tiles * (D / 64) * 4), 2), 256, 0, stream>>>(j);
+}
 
 }  // namespace fa2

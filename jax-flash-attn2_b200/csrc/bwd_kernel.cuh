@@ -163,7 +163,9 @@ bwd_dq_convert(const float* __restrict__ dq_acc, uint16_t* __restrict__ dq, long
 // 2. main kernel
 // ---------------------------------------------------------------------------------------------
 // kMod: kNoMod, or the score changes of a scored kernel (score_mod.cuh); those take causal masking from p.mod.
-template <int D, bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod>
+// kParts: blockIdx.y takes a part of the query heads (BwdKernelParams::part_kv). A kernel of its own, since as a branch of the
+// epilogue it slowed the capped kernel by 4 to 10 % though neither spills nor registers changed.
+template <int D, bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod, bool kParts = false>
 __global__ void __launch_bounds__(BwdRoles<D>::kThreads, 1)
 bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -232,7 +234,9 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   int i_end = nQ_b;
   if constexpr (kScored) key_tile_range<kBM>(p.mod, b, n, p.Sq, p.causal_off, i_start, i_end);
   const int nI = i_end - i_start;                    // query tiles per head
-  const int T = (n * kBN < sk_b) ? nI * p.G : 0;     // steps of this CTA (none: dK = dV = 0)
+  const int heads = kParts ? p.G / static_cast<int>(gridDim.y) : p.G;      // query heads of this CTA
+  const int h0 = hk * p.G + (kParts ? static_cast<int>(blockIdx.y) * heads : 0);
+  const int T = (n * kBN < sk_b) ? nI * heads : 0;   // steps of this CTA (none: dK = dV = 0)
   const bool dead_keys = n * kBN + kBN > sk_b;       // some key rows lie past the end
 
   if (tid == 0) {
@@ -294,7 +298,7 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   auto step_coords = [&](int it, int& h, int& i) {
     const int g = it / nI;
     i = i_start + (it - g * nI);
-    h = hk * p.G + g;
+    h = h0 + g;
   };
 
   if constexpr (kPW == 2) {
@@ -893,6 +897,10 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
           for (int k = 0; k < 32; ++k) a[k] = 0u;
         }
+        if constexpr (kParts) {
+          store_part_columns(part_tile<D>(p, acc, bhk, n), c * 8, r, a, f);
+          continue;
+        }
         uint8_t* line = stage + (c >> 1) * L::kBlockBytes + r * 128;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
@@ -908,7 +916,7 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       fence_proxy_async_smem();
     }
     named_bar_sync(1 + acc, 128 * kWgPerAcc);
-    if (ok && part == 0 && r == 0 && !*abort_flag) {
+    if (ok && part == 0 && r == 0 && !*abort_flag && !kParts) {
       tma_store_5d(acc == 0 ? &tmdK : &tmdV, sQ + acc * L::kTileBytes, 0, n * kBN, 0, hk, b);
       tma_store_commit();
       tma_store_wait_read0();
@@ -927,15 +935,15 @@ bwd_main_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 // ---------------------------------------------------------------------------------------------
 // launcher
 // ---------------------------------------------------------------------------------------------
-template <int D, bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod>
+template <int D, bool kBf16, bool kCausal, bool kFeat, int kMod = kNoMod, bool kParts = false>
 static cudaError_t launch_main(const BwdLaunch& a, cudaStream_t stream) {
   using L = BwdSmem<D, kFeat && D == 64>;
-  auto kern = bwd_main_kernel<D, kBf16, kCausal, kFeat, kMod>;
+  auto kern = bwd_main_kernel<D, kBf16, kCausal, kFeat, kMod, kParts>;
   static bool smem_opted_in[64] = {};
   cudaError_t e = opt_in_dynamic_smem(kern, L::kDynamicBytes, smem_opted_in);
   if (e != cudaSuccess) return e;
   const long long nblocks = static_cast<long long>(a.kp.n_kvblk) * a.kp.B * a.kp.Hkv;
-  kern<<<static_cast<unsigned>(nblocks), BwdRoles<D>::kThreads, L::kDynamicBytes, stream>>>(
+  kern<<<dim3(static_cast<unsigned>(nblocks), a.parts), BwdRoles<D>::kThreads, L::kDynamicBytes, stream>>>(
       a.tmQ, a.tmK, a.tmV, a.tmdO, a.tmdK, a.tmdV, a.tmBias, a.tmMask, a.delta, a.kp);
   return cudaGetLastError();
 }
@@ -971,6 +979,7 @@ static cudaError_t launch_passes(const BwdLaunch& a, cudaStream_t stream, Main m
                                                      a.dq_strides[0], a.dq_strides[1],
                                                      a.dq_strides[2], kp.Sq, kp.Hq, nQ, kp.scale,
                                                      kBf16 ? nullptr : kp.do_absmax_bits, a.head_blk);
+  if (kp.part_kv != nullptr) launch_kv_join<D, kBf16>(a, stream);
   mark(3);
   return cudaGetLastError();
 }

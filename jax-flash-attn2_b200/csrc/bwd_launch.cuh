@@ -20,6 +20,8 @@ struct BwdLaunch {
   const void* o;   long long o_strides[3];    // (batch, sequence, head) element strides
   const void* d_o; long long do_strides[3];
   void* dq;        long long dq_strides[3];
+  int parts;       // 1, or the parts of the query heads of a key/value head (BwdKernelParams::part_kv)
+  void *dk, *dv;   long long dk_strides[3], dv_strides[3];   // read with more than one part alone
   float* delta;    // start of the row-statistics area of the workspace
   size_t dq_acc_bytes;
   // Optional: recorded before the pre-pass, before the main kernel, after it, after the dq

@@ -3,15 +3,20 @@
 
 namespace fa2 {
 
+template <bool kBf16, bool kParts>
+static cudaError_t launch_mod(const BwdLaunch& a, int mod, cudaStream_t stream) {
+  switch (mod) {
+    case 0: return launch_main<128, kBf16, false, false, 0, kParts>(a, stream);
+    case 1: return launch_main<128, kBf16, false, false, 1, kParts>(a, stream);
+    case 2: return launch_main<128, kBf16, false, false, 2, kParts>(a, stream);
+    default: return launch_main<128, kBf16, false, false, 3, kParts>(a, stream);
+  }
+}
+
 template <bool kBf16>
 static cudaError_t launch_scored(const BwdLaunch& a, int mod, cudaStream_t stream) {
   return launch_passes<128, kBf16>(a, stream, [mod](const BwdLaunch& l, cudaStream_t s) {
-    switch (mod) {
-      case 0: return launch_main<128, kBf16, false, false, 0>(l, s);
-      case 1: return launch_main<128, kBf16, false, false, 1>(l, s);
-      case 2: return launch_main<128, kBf16, false, false, 2>(l, s);
-      default: return launch_main<128, kBf16, false, false, 3>(l, s);
-    }
+    return l.parts > 1 ? launch_mod<kBf16, true>(l, mod, s) : launch_mod<kBf16, false>(l, mod, s);
   });
 }
 

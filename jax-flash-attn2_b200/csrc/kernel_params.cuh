@@ -166,6 +166,10 @@ struct BwdKernelParams {
   int* dq_order;
   int* status;
   ScoreModDev mod;      // read by the scored kernels alone
+  // Scored kernels on a grid of (key tiles, parts): part y takes its share of the query heads of a key/value head
+  // and leaves dK and dV in float32, [part][dK, dV][B * Hkv * n_kvblk][kernel head dim / 4][128 keys][4]
+  // (bwd_kv_join_kernel); null: one part, which writes them itself.
+  float* part_kv;
 };
 
 }  // namespace fa2

@@ -35,6 +35,7 @@ LM_EXPORTED_SYMBOLS = (
     "fa2_document_layout_bytes",
     "fa2_document_layout",
     "fa2_scored_fwd",
+    "fa2_scored_bwd_workspace_bytes",
     "fa2_scored_bwd",
     "fa2_paged_work_bytes",
     "fa2_paged_plan",
@@ -46,7 +47,7 @@ FA2_BWD_STATIC_SCRATCH_BYTES = 32 * 1024 * 1024
 # FA2_ABI_VERSION of the header these structures were written against (major * 1000 + minor)
 FA2_ABI_VERSION = 3000
 # the same for fa2_b200_lm.h
-FA2_LM_ABI_VERSION = 1000
+FA2_LM_ABI_VERSION = 1001
 
 
 class Strides(C.Structure):
@@ -259,6 +260,8 @@ def load() -> C.CDLL:
     lib.fa2_document_layout.restype = C.c_int
     lib.fa2_scored_fwd.argtypes = [C.POINTER(FwdParams), C.POINTER(ScoreMod), C.c_void_p]
     lib.fa2_scored_fwd.restype = C.c_int
+    lib.fa2_scored_bwd_workspace_bytes.argtypes = [C.POINTER(Problem)]
+    lib.fa2_scored_bwd_workspace_bytes.restype = C.c_size_t
     lib.fa2_scored_bwd.argtypes = [C.POINTER(BwdParams), C.POINTER(ScoreMod), C.c_void_p]
     lib.fa2_scored_bwd.restype = C.c_int
     lib.fa2_paged_work_bytes.argtypes = [C.c_int32] * 4

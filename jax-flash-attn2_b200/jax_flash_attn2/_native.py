@@ -7,7 +7,7 @@ from . import _capi
 
 # the functions the module calls, in the order of its `Abi`
 _FUNCTIONS = (
-    "fa2_document_layout_bytes", "fa2_document_layout", "fa2_fwd_workspace_bytes", "fa2_bwd_workspace_bytes",
+    "fa2_document_layout_bytes", "fa2_document_layout", "fa2_fwd_workspace_bytes", "fa2_scored_bwd_workspace_bytes",
     "fa2_scored_fwd", "fa2_scored_bwd", "fa2_paged_work_bytes", "fa2_paged_plan", "fa2_paged_cache_write",
     "fa2_paged_workspace_bytes", "fa2_paged_attention", "fa2_last_error",
 )

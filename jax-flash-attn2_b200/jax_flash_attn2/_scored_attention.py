@@ -183,7 +183,8 @@ def bwd_scored_attention_kernel_call(
     dv = torch.empty_like(v, memory_format=torch.contiguous_format)
     a = _capi.BwdParams()
     a.p = _problem(q, k, softmax_scale, 0.0, causal, None, 0, 0, None)
-    nbytes = lib.fa2_bwd_workspace_bytes(C.byref(a.p))
+    with torch.cuda.device(q.device):
+        nbytes = lib.fa2_scored_bwd_workspace_bytes(C.byref(a.p))
     if nbytes == 0:
         _capi.check(_capi.FA2_ERR_INVALID_ARG)
     workspace = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)

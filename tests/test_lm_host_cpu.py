@@ -297,3 +297,21 @@ def test_serving_calls_take_no_part_in_training():
     assert y._version == 1
     with torch.inference_mode():
         J._paged._written(torch.zeros(2))
+
+
+@pytest.mark.parametrize("shape,parts", [
+    ((1, 512, 512, 32, 8, 128), 4), ((1, 1024, 1024, 32, 8, 64), 2), ((1, 512, 512, 12, 2, 64), 6), ((1, 512, 512, 20, 4, 256), 1),
+    ((1, 512, 512, 24, 4, 256), 3), ((4, 4096, 4096, 32, 8, 128), 1), ((1, 128, 128, 8, 4, 64), 1), ((1, 256, 128, 8, 4, 64), 2),
+    ((1, 64, 64, 8, 8, 64), 1),
+])
+def test_parts_of_the_query_heads(shape, parts):
+    # 148 SMs are assumed where there is no device
+    if torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("written for 148 SMs")
+    p = _capi.Problem()
+    p.batch, p.seqlen_q, p.seqlen_k, p.heads_q, p.heads_kv, p.head_dim = shape
+    p.heads_q_global, p.dtype, p.causal, p.softmax_scale = p.heads_q, _capi.FA2_BF16, 1, 0.1
+    lib = _capi.load()
+    more = lib.fa2_scored_bwd_workspace_bytes(C.byref(p)) - lib.fa2_bwd_workspace_bytes(C.byref(p))
+    tiles = shape[0] * shape[4] * ((shape[2] + 127) // 128)
+    assert more == (parts * 2 * tiles * 128 * shape[5] * 4 if parts > 1 else 0)

@@ -333,3 +333,36 @@ def test_some_operands_without_gradients_and_operands_to_be_copied():
         J.scored_flash_attention(q, k, v, softcap=-1.0)
     with pytest.raises(AssertionError, match="fp16 and bf16"):
         J.scored_flash_attention(q.float(), k.float(), v.float())
+
+
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hkv,D,dtype,docs", [
+    (1, 300, 300, 8, 2, 64, BF16, False), (1, 300, 300, 8, 1, 128, FP16, True), (2, 200, 330, 6, 2, 256, BF16, False),
+    (1, 515, 515, 12, 2, 96, BF16, True), (1, 129, 1, 8, 1, 40, FP16, False), (3, 257, 257, 4, 2, 160, FP16, True),
+])
+def test_query_heads_in_parts_and_in_one(B, Sq, Sk, Hq, Hkv, D, dtype, docs, monkeypatch):
+    """The backward deals the query heads to several SMs where there are few key tiles (more scratch): against the formulas
+    with and without, dq the same bits."""
+    import ctypes as C
+    import jax_flash_attn2 as J
+    from jax_flash_attn2 import _capi, _kernel_calls
+    lib = _capi.load()
+    q, k, v, do = W.make_qkv(B, Sq, Sk, Hq, Hkv, D, dtype)
+    ids = ids_of([[(0, Sq // 3), (1, Sq // 2)]] * B, Sq) if docs else None
+    want = O.attention(q, k, v, O.visible_keys(B, Sq, Sk, True, ids), None, 20.0, slopes_of(Hq), do)
+    bound = O.bounds(want, dtype)
+    dq, dk, dv, ddo = (x.cuda() for x in (q, k, v, do))
+    problem = _kernel_calls._problem(dq, dk, None, 0.0, True, None, 0, 0, None)
+    assert lib.fa2_scored_bwd_workspace_bytes(C.byref(problem)) > lib.fa2_bwd_workspace_bytes(C.byref(problem))
+    rest = torch.empty_like(dq)
+    kw = dict(softcap=20.0, alibi_slopes=slopes_of(Hq).cuda(), layout=J.document_layout(ids.cuda()) if docs else None, rest=rest)
+    out, lse = J.fwd_scored_attention_kernel_call(dq, dk, dv, None, True, **kw)
+    run = lambda: J.bwd_scored_attention_kernel_call(ddo, dq, dk, dv, out, lse, None, True, deterministic=True, **kw)
+    parts, again = run(), run()
+    assert all(torch.equal(x, y) for x, y in zip(parts, again))
+    monkeypatch.setattr(lib, "fa2_scored_bwd_workspace_bytes", lib.fa2_bwd_workspace_bytes)
+    one = run()
+    assert torch.equal(one[0], parts[0])
+    for grads in (parts, one):
+        for name, x in zip(("dq", "dk", "dv"), grads):
+            assert O.worst(x, want[name], bound[name]) <= 1.0, name
+    assert J.device_status() == 0
