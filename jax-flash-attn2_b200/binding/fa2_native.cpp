@@ -96,6 +96,15 @@ Tensor bytes_like(const Tensor& x, size_t n) {
   return at::empty({static_cast<int64_t>(n)}, x.options().dtype(at::kByte));
 }
 
+// `n` elements of type `t` from byte `at` of a fresh buffer, as a tensor of their own.
+Tensor part_of(const Tensor& buffer, at::ScalarType t, int64_t at, int64_t n) {
+  Tensor x = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(),
+                                                      c10::scalarTypeToTypeMeta(t));
+  x.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(t)));
+  x.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return x;
+}
+
 // Tells autograd of a write in place, so that a backward pass that saved `x` notices.
 void written(const Tensor& x) {
   if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
@@ -354,11 +363,14 @@ PyObject* paged_step_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const size_t bytes = abi.paged_work_bytes(static_cast<int32_t>(requests), static_cast<int32_t>(tokens),
                                             static_cast<int32_t>(heads_q), static_cast<int32_t>(heads_kv));
   if (bytes == 0) Py_RETURN_NONE;
-  const int64_t ints = static_cast<int64_t>(bytes / 4);
-  const auto options = table.options();
-  const Tensor work = at::empty({ints}, options), cu = at::empty({requests + 1}, options), lens = at::empty({requests}, options),
-               positions = at::empty({tokens}, options), taken = at::empty({1}, options),
-               slots = at::empty({tokens}, options.dtype(at::kLong));
+  // one buffer for all of it (an allocation takes longer on the host than a tensor on top of one): the work list, whose size is
+  // a multiple of 16 bytes, the slots, and the int32 arrays
+  const int64_t slots_at = static_cast<int64_t>((bytes + 15) / 16 * 16), cu_at = slots_at + 8 * tokens,
+                lens_at = cu_at + 4 * (requests + 1), positions_at = lens_at + 4 * requests, taken_at = positions_at + 4 * tokens;
+  const Tensor buffer = bytes_like(table, static_cast<size_t>(taken_at + 4));
+  const Tensor work = part_of(buffer, at::kInt, 0, static_cast<int64_t>(bytes / 4)), slots = part_of(buffer, at::kLong, slots_at, tokens),
+               cu = part_of(buffer, at::kInt, cu_at, requests + 1), lens = part_of(buffer, at::kInt, lens_at, requests),
+               positions = part_of(buffer, at::kInt, positions_at, tokens), taken = part_of(buffer, at::kInt, taken_at, 1);
   fa2_paged_plan_params a = {};
   a.context_lens = context.const_data_ptr<int32_t>();
   a.new_lens = fresh.const_data_ptr<int32_t>();
