@@ -419,3 +419,30 @@ def test_writes_in_place_are_known_to_autograd():
     plan.block_table = table.long()
     with pytest.raises(ValueError, match="paged_step_plan"):
         J.paged_attention(out.detach(), cache, other, plan)
+
+
+@pytest.mark.parametrize("requests", [4097, 5000])
+def test_more_items_than_the_plan_keeps_in_shared_memory(requests):
+    import jax_flash_attn2 as J
+    g = torch.Generator().manual_seed(requests)
+    page, width, Hq, Hkv, D = 8, 6, 4, 2, 64
+    context = torch.randint(0, page * width - 1, (requests,), generator=g, dtype=torch.int32)
+    pages = requests * width
+    table = torch.randperm(pages, generator=g).to(torch.int32).view(requests, width)
+    kc, vc = (torch.randn(pages, page, Hkv, D, generator=g).to(BF16) for _ in range(2))
+    q = torch.randn(requests, Hq, D, generator=g).to(BF16)
+    # (pages that the new tokens open are taken from the same pool: some page may serve two requests, which changes nothing here)
+    plan = J.paged_step_plan(context.cuda(), torch.ones_like(context).cuda(), table.cuda(), table.flatten().cuda(), page_size=page,
+                             num_tokens=requests, heads_q=Hq, heads_kv=Hkv)
+    assert torch.equal(plan.seqlens_k.cpu(), context + 1)
+    used = plan.block_table.cpu()
+    out = J.paged_attention(q.cuda(), kc.cuda(), vc.cuda(), plan).cpu()
+    assert J.device_status() == 0
+    k, v = (x[used.long()].reshape(requests, page * width, Hkv, D).double() for x in (kc, vc))
+    s = torch.einsum("rhgd,rjhd->rhgj", q.double().view(requests, Hkv, Hq // Hkv, D), k) / D ** 0.5
+    seen = torch.arange(page * width) <= context[:, None]
+    p = torch.softmax(s.masked_fill(~seen[:, None, None], -torch.inf), -1)
+    want = torch.einsum("rhgj,rjhd->rhgd", p, v).reshape(requests, Hq, D)
+    # half a step for the weights, half a step for the output, a hundredth of that for sums in 32 bits and the exponential
+    size = torch.einsum("rhgj,rjhd->rhgd", p, v.abs()).reshape(requests, Hq, D)
+    assert torch.all((out.double() - want).abs() <= 2.02 * 2 ** -8 * size + 1e-6)
