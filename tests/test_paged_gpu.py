@@ -446,3 +446,30 @@ def test_more_items_than_the_plan_keeps_in_shared_memory(requests):
     # half a step for the weights, half a step for the output, a hundredth of that for sums in 32 bits and the exponential
     size = torch.einsum("rhgj,rjhd->rhgd", p, v.abs()).reshape(requests, Hq, D)
     assert torch.all((out.double() - want).abs() <= 2.02 * 2 ** -8 * size + 1e-6)
+
+
+def test_a_pool_of_more_than_2_31_elements():
+    import jax_flash_attn2 as J
+    g = torch.Generator().manual_seed(3)
+    page, Hq, Hkv, D, used = 16, 4, 2, 64, 40
+    pages = 2 ** 31 // (page * Hkv * D) + used
+    context, new = [300, 17], [40, 1]
+    small = [torch.randn(used, page, Hkv, D, generator=g).to(BF16).cuda() for _ in range(2)]
+    large = [torch.empty(pages, page, Hkv, D, dtype=BF16, device="cuda") for _ in range(2)]
+    for a, b in zip(large, small):
+        a[-used:] = b
+    assert large[0][-1].data_ptr() - large[0].data_ptr() > 2 * 2 ** 31
+    q = torch.randn(sum(new), Hq, D, generator=g).to(BF16).cuda()
+    k, v = (torch.randn(sum(new), Hkv, D, generator=g).to(BF16).cuda() for _ in range(2))
+    order = torch.randperm(used, generator=g).to(torch.int32)
+    outs = []
+    for first, caches in ((0, small), (pages - used, large)):
+        table = torch.full((2, 24), -1, dtype=torch.int32)
+        table[0, :19] = order[:19] + first
+        table[1, :2] = order[19:21] + first
+        plan = J.paged_step_plan(dev_int(context), dev_int(new), table.cuda(), (order[21:] + first).cuda(), page_size=page,
+                                 num_tokens=sum(new), heads_q=Hq, heads_kv=Hkv)
+        J.paged_cache_write(k, v, *caches, plan.slot_map)
+        outs.append(J.paged_attention(q, *caches, plan))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(small[0], large[0][-used:]) and torch.equal(small[1], large[1][-used:])
+    assert torch.isfinite(outs[0].float()).all() and J.device_status() == 0

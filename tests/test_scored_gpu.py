@@ -366,3 +366,53 @@ def test_query_heads_in_parts_and_in_one(B, Sq, Sk, Hq, Hkv, D, dtype, docs, mon
         for name, x in zip(("dq", "dk", "dv"), grads):
             assert O.worst(x, want[name], bound[name]) <= 1.0, name
     assert J.device_status() == 0
+
+
+def test_tensors_of_more_than_2_31_elements():
+    """Packed documents of 128 tokens: the last ones are the same problem as a short call."""
+    import jax_flash_attn2 as J
+    S, Hq, Hkv, D, tail = 2 ** 17 + 2 ** 11, 130, 1, 128, 1024
+    g = torch.Generator(device="cuda").manual_seed(4)
+    make = lambda h: torch.randn(1, S, h, D, generator=g, device="cuda", dtype=BF16)
+    q, k, v, do = make(Hq), make(Hkv), make(Hkv), make(Hq)
+    assert q.numel() > 2 ** 31
+    ids = (torch.arange(S, device="cuda", dtype=torch.int32) // 128)[None]
+
+    def run(q, k, v, do, ids):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = J.scored_flash_attention(*leaves, None, True, softcap=20.0, document_ids=ids)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    got = [x[:, -tail:].clone() for x in run(q, k, v, do, ids)]
+    want = run(*(x[:, -tail:].contiguous() for x in (q, k, v, do, ids)))
+    assert J.device_status() == 0
+    # one key tile takes part in a row of dq, so that only the sums of dk and dv over the heads may be in another order:
+    # half a step of the result and the sums of 130 heads x 128 queries in 32 bits
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for x, y in zip(got[2:], want[2:]):
+        x, y = x.double(), y.double()
+        assert torch.all((x - y).abs() <= 2 * 2 ** -8 * y.abs() + 2e-3 * y.abs().mean())
+
+
+def test_batch_rows_far_apart():
+    import jax_flash_attn2 as J
+    shape, step = (2, 200, 2, 64), 2 ** 31 + 64
+    near = W.make_qkv(2, 200, 200, 2, 2, 64, BF16)
+    room = torch.empty(step + 200 * 2 * 64, dtype=BF16, device="cuda")
+    base = [x.cuda().requires_grad_(True) for x in near[:3]]
+    want = J.scored_flash_attention(*base, None, True, softcap=20.0)
+    grads = torch.autograd.grad(want, base, near[3].cuda())
+    far = torch.as_strided(room, shape, (step, 128, 64, 1))
+    for which in range(3):
+        with torch.no_grad():
+            far.copy_(base[which])
+        leaves = list(base)
+        leaves[which] = far.detach().requires_grad_(True)
+        out = J.scored_flash_attention(*leaves, None, True, softcap=20.0)
+        assert torch.equal(out, want)
+        assert torch.equal(torch.autograd.grad(out, leaves, near[3].cuda())[2], grads[2])
+    with torch.no_grad():
+        far.copy_(near[3])
+    out = J.scored_flash_attention(*base, None, True, softcap=20.0)
+    assert torch.equal(torch.autograd.grad(out, base, far)[1], grads[1])
+    assert J.device_status() == 0
