@@ -22,8 +22,10 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/autograd.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "../../include/fa2_b200_lm.h"
@@ -176,46 +178,50 @@ Tensor laid_out(const Tensor& x) {
   return fine ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
-struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
-                        Scored* s, bool* refused) {
-    // bf16: see o_rest in fa2_b200_lm.h
-    if (q.scalar_type() == at::kBFloat16) s->rest = at::empty(q.sizes(), q.options());
-    Tensor out, lse;
-    *refused = !forward_launch(q, k, v, *s, &out, &lse);
-    ctx->save_for_backward({q, k, v, out, lse, s->slopes, s->layout, s->prefix, s->rest});
-    ctx->saved_data["scale"] = s->scale;
-    ctx->saved_data["softcap"] = s->softcap;
-    ctx->saved_data["causal"] = s->causal;
-    return out;
+// The backward pass as a node of the autograd graph. Written out (torch::autograd::Function would do) because at a few
+// hundred tokens autograd's work on the host is what a training step takes: lse and rest never leave the node.
+struct ScoredBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable q, k, v, out, slopes, layout, prefix;
+  Tensor lse, rest;
+  double scale = 0, softcap = 0;
+  bool causal = false;
+
+  std::string name() const override { return "ScoredAttentionBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto* x : {&q, &k, &v, &out, &slopes, &layout, &prefix}) x->reset_data();
+    lse.reset();
+    rest.reset();
   }
 
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
-                                                 torch::autograd::variable_list grads) {
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     TORCH_CHECK(!at::GradMode::is_enabled(), "scored_flash_attention has no second derivatives (create_graph=True)");
-    torch::autograd::variable_list result(5);
+    torch::autograd::variable_list result(3);
     if (!grads[0].defined()) return result;
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4];
+    const Tensor inputs[3] = {q.unpack(), k.unpack(), v.unpack()};
+    const Tensor o = out.unpack(shared_from_this());
     Scored s;
-    s.slopes = saved[5];
-    s.layout = saved[6];
-    s.prefix = saved[7];
-    s.rest = saved[8];
-    s.scale = ctx->saved_data["scale"].toDouble();
-    s.softcap = ctx->saved_data["softcap"].toDouble();
-    s.causal = ctx->saved_data["causal"].toBool();
-    const c10::cuda::CUDAGuard guard(q.device());
+    s.slopes = slopes.unpack();
+    s.layout = layout.unpack();
+    s.prefix = prefix.unpack();
+    s.rest = rest;
+    s.scale = scale;
+    s.softcap = softcap;
+    s.causal = causal;
+    const at::AutoDispatchBelowADInplaceOrView no_autograd;
+    const c10::cuda::CUDAGuard guard(o.device());
     const Tensor d_o = laid_out(grads[0]);
     fa2_bwd_params a = {};
-    a.p = problem_of(q, k, s);
+    a.p = problem_of(inputs[0], inputs[1], s);
     const size_t n = abi.scored_bwd_workspace_bytes(&a.p);
-    const Tensor workspace = bytes_like(q, n);
-    for (int i = 0; i < 3; ++i) result[i] = at::empty(saved[i].sizes(), q.options());
-    a.q = q.const_data_ptr(); a.q_strides = strides_of(q);
-    a.k = k.const_data_ptr(); a.k_strides = strides_of(k);
-    a.v = v.const_data_ptr(); a.v_strides = strides_of(v);
-    a.o = out.const_data_ptr(); a.o_strides = strides_of(out);
+    const Tensor workspace = bytes_like(o, n);
+    for (int i = 0; i < 3; ++i) result[i] = at::empty(inputs[i].sizes(), o.options());
+    a.q = inputs[0].const_data_ptr(); a.q_strides = strides_of(inputs[0]);
+    a.k = inputs[1].const_data_ptr(); a.k_strides = strides_of(inputs[1]);
+    a.v = inputs[2].const_data_ptr(); a.v_strides = strides_of(inputs[2]);
+    a.o = o.const_data_ptr(); a.o_strides = strides_of(o);
     a.d_o = d_o.const_data_ptr(); a.do_strides = strides_of(d_o);
     a.lse = lse.const_data_ptr<float>();
     a.lse_stride_b = lse.stride(0);
@@ -229,11 +235,36 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     a.deterministic = det && *det && !(det[0] == '0' && det[1] == 0);
     fa2_score_mod m;
     s.fill(&m);
-    const int rc = abi.scored_bwd(&a, &m, stream_of(q));
+    const int rc = abi.scored_bwd(&a, &m, stream_of(o));
     TORCH_CHECK(rc == FA2_OK, "fa2_b200 error ", rc, ": ", abi.last_error());
     return result;
   }
 };
+
+// The forward pass under autograd; false if the library refused the call.
+bool forward_with_node(const Tensor& q, const Tensor& k, const Tensor& v, Scored* s, Tensor* out) {
+  const std::shared_ptr<ScoredBackward> node(new ScoredBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
+  {
+    const at::AutoDispatchBelowADInplaceOrView no_autograd;
+    // bf16: see o_rest in fa2_b200_lm.h
+    if (q.scalar_type() == at::kBFloat16) node->rest = s->rest = at::empty(q.sizes(), q.options());
+    if (!forward_launch(q, k, v, *s, out, &node->lse)) return false;
+  }
+  torch::autograd::set_history(*out, node);
+  using torch::autograd::SavedVariable;
+  node->q = SavedVariable(q, false);
+  node->k = SavedVariable(k, false);
+  node->v = SavedVariable(v, false);
+  node->out = SavedVariable(*out, true);
+  node->slopes = SavedVariable(s->slopes, false);
+  node->layout = SavedVariable(s->layout, false);
+  node->prefix = SavedVariable(s->prefix, false);
+  node->scale = s->scale;
+  node->softcap = s->softcap;
+  node->causal = s->causal;
+  return true;
+}
 
 // Whether a live autograd graph made on another stream ends in the leaf `x`: autograd would synchronise with that stream,
 // which breaks a capture.
@@ -322,7 +353,7 @@ PyObject* scored_flash_attention(PyObject*, PyObject* const* args, Py_ssize_t n)
     }
     if (!refused) {
       if (grad) {
-        out = ScoredAttention::apply(q, k, v, &s, &refused);
+        refused = !forward_with_node(q, k, v, &s, &out);
       } else {
         Tensor lse;
         refused = !forward_launch(q, k, v, s, &out, &lse);

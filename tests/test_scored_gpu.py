@@ -416,3 +416,39 @@ def test_batch_rows_far_apart():
     out = J.scored_flash_attention(*base, None, True, softcap=20.0)
     assert torch.equal(torch.autograd.grad(out, base, far)[1], grads[1])
     assert J.device_status() == 0
+
+
+def test_graph_bookkeeping():
+    """Second passes, changed operands, hooks and several consumers behave as for other torch operators."""
+    import jax_flash_attn2 as J
+    q, k, v, do = (x.cuda() for x in W.make_qkv(1, 70, 70, 2, 2, 64, BF16))
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    prefix = torch.tensor([5], dtype=torch.int32, device="cuda")
+    f = lambda: J.scored_flash_attention(*leaves, None, True, softcap=20.0, prefix_lens=prefix)
+    out = f()
+    assert out.requires_grad and out.grad_fn.name() == "ScoredAttentionBackward" and not out.is_leaf
+    first = torch.autograd.grad(out, leaves, do, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, do)
+    assert all(torch.equal(x, y) for x, y in zip(first, second))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, leaves, do)
+    for what in ("prefix", "out"):
+        out = f()
+        with torch.no_grad():
+            (prefix if what == "prefix" else out).add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaves, do)
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: packed.append(x.shape) or x.cpu(), lambda x: x.cuda()):
+        out = f()
+    assert len(packed) >= 4
+    assert all(torch.equal(x, y) for x, y in zip(first, torch.autograd.grad(out, leaves, do)))
+    # two layers on one input, and no gradient asked for one operand
+    a = f() + f()
+    assert torch.equal(torch.autograd.grad(a, leaves[1], do)[0], 2 * first[1])
+    # gradients that are accumulated into
+    f().backward(do)
+    f().backward(do)
+    assert torch.equal(leaves[2].grad, 2 * first[2])
+    out = f()
+    assert torch.autograd.grad(out.sum() * 0 + leaves[0].sum() * 0, leaves[0])[0].abs().max() == 0
