@@ -11,8 +11,8 @@ cudaError_t launch_document_layout(const int* ids, long long stride_b, int B, in
 
 // Work list of the paged attention (int32):
 //   header     kWorkHeader words: 0: items, 1: CTAs that get a share
-//   starts     where every CTA starts and, behind the last one, the end: 4 words (key/value head, item, key tile, 0) for each
-//              of the device's SMs and one more
+//   starts     where every CTA starts and, behind the last one, the end: 4 words (key/value head, item, key tile, 1 if it
+//              starts inside an item of two query tiles) for each of the device's SMs and one more
 //   items      kWorkItem words each: first row of the packed tensors, tokens, position of the first token, request, cost of
 //              the items before it, key tiles of its own, cost of a key tile (1 or 2), 0
 constexpr int kWorkHeader = 16;

@@ -59,10 +59,11 @@ struct PagedSmem {
   static_assert(kDynamicBytes <= 232448, "shared memory budget exceeded");
 };
 
-// A CTA's way from its start to the next CTA's. An item it begins inside of comes last, so that the CTAs, which all begin with
-// the first key tile of some item, walk over the keys of a long request side by side and share them in L2: 4096 new tokens of
-// 64/8 heads, D = 128, over 65536 keys 8.55 -> 7.77 ms, over 32768 3.75 -> 3.67, over 8192 (which fit L2 either way)
-// 0.678 -> 0.690.
+// A CTA's way from its start to the next CTA's. An item of two query tiles (part of a chunk, whose other items see the same
+// keys) that it begins inside of comes last, so that the CTAs, which all begin with the first key tile of some item, walk over
+// the keys of a long request side by side and share them in L2: 4096 new tokens of 64/8 heads, D = 128, over 65536 keys 8.55 ->
+// 7.77 ms, over 32768 3.75 -> 3.67, over 8192 (which fit L2 either way) 0.678 -> 0.690. Single tokens share nothing, and are
+// faster in the order of the line (64 over 2464 keys 135 us, 142 with the first piece last).
 struct PagedWalk {
   int n_items;
   int hk, i, tile;
@@ -109,7 +110,7 @@ __device__ __forceinline__ void paged_start(const PagedAttnDev& p, PagedWalk& w)
   const int4 from = paged_start_of(p.work, c), to = paged_start_of(p.work, c + 1);
   w.hk = from.x; w.i = from.y; w.tile = from.z;
   w.end_hk = to.x; w.end_i = to.y; w.end_tile = to.z;
-  if (w.tile > 0 && (w.hk != w.end_hk || w.i != w.end_i)) {
+  if (from.w != 0 && w.tile > 0 && (w.hk != w.end_hk || w.i != w.end_i)) {
     w.late = 1;
     w.tile = 0;
     paged_advance(w);

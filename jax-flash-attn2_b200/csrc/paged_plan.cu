@@ -210,7 +210,7 @@ paged_plan_kernel(const PagedPlanDev p) {
       int tile = (in + cost - 1) / cost;
       if (in <= snap && in <= left) tile = 0;
       else if (left <= snap) tile = item.y;
-      start = make_int4(hk, lo, tile, 0);
+      start = make_int4(hk, lo, tile, cost == 2);
       if (tile >= item.y) start = lo + 1 < n_items ? make_int4(hk, lo + 1, 0, 0) : make_int4(hk + 1, 0, 0, 0);
     }
     reinterpret_cast<int4*>(p.work + kWorkHeader)[c] = start;
