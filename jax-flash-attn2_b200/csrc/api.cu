@@ -666,8 +666,8 @@ int fa2_paged_plan(const fa2_paged_plan_params* a, void* cuda_stream) {
   if (a->work_bytes < (work_items_at(sm_count()) + kWorkItem * static_cast<size_t>(items)) * sizeof(int32_t))
     return fail(FA2_ERR_WORKSPACE, "work must hold fa2_paged_work_bytes bytes");
   const int64_t tiles = ((static_cast<int64_t>(a->table_width) << shift) + 127) / 128;
-  if (2 * items * (tiles + 2) > INT_MAX)
-    return fail(FA2_ERR_UNSUPPORTED, "problem too large: %lld items of up to %lld key tiles must stay below 2^30",
+  if (items * (kTileCost2 * tiles + kItemCost2) > INT_MAX)
+    return fail(FA2_ERR_UNSUPPORTED, "problem too large: %lld items of up to %lld key tiles must stay below 2^29",
                 static_cast<long long>(items), static_cast<long long>(tiles));
   PagedPlanDev d;
   d.context_lens = a->context_lens;

@@ -14,9 +14,13 @@ cudaError_t launch_document_layout(const int* ids, long long stride_b, int B, in
 //   starts     where every CTA starts and, behind the last one, the end: 4 words (key/value head, item, key tile, 1 if it
 //              starts inside an item of two query tiles) for each of the device's SMs and one more
 //   items      kWorkItem words each: first row of the packed tensors, tokens, position of the first token, request, cost of
-//              the items before it, key tiles of its own, cost of a key tile (1 or 2), 0
+//              the items before it, key tiles of its own, cost of a key tile, 0
 constexpr int kWorkHeader = 16;
 constexpr int kWorkItem = 8;
+// What the plan deals out in equal shares: the cost of a key tile of an item of one query tile and of two, and of the start and
+// end of such an item. (From clock readings of every CTA, fitted: a key tile 2.1 and 2.9 thousand cycles at D = 64, 2.7 and
+// 3.8 at D = 128, a start and end 5.3 and 5.9, 7.4 and 12.5; where memory is the bound, single tokens take less of both.)
+constexpr int kTileCost1 = 2, kTileCost2 = 3, kItemCost1 = 4, kItemCost2 = 8;
 inline int work_items_at(int sms) { return kWorkHeader + (4 * (sms + 1) + 7) / 8 * 8; }   // word of the first item
 
 struct PagedPlanDev {

@@ -6,12 +6,13 @@
 //   fresh_b = sum over the requests before b of need - have: its pages in the list of free ones start there
 //   token i of it: position c_b + i, slot = page(position >> s) * 2^s + position mod 2^s
 // and the work list of the attention: items of `item_tokens` query tokens with the number of 128-key tiles that each
-// of them sees and what such a tile costs (2 if the tokens need both query tiles, else 1). All tiles of all items of all
-// key/value heads form a line as long as their costs (an item begins with the cost of two of its tiles, which is what
-// its start and its end take), which is cut into equal shares, one per SM. A border that falls next to
+// of them sees. All tiles of all items of all key/value heads form a line as long as their costs (lm_launch.cuh; an item
+// begins with the cost of its start and end), which is cut into equal shares, one per SM. A border that falls next to
 // an end of an item moves to that end, by at most snap_of (and half a share): an item that is cut costs partial rows of both
 // sides, written and joined, about as much as two tiles of 256 rows or half a tile of a few.
-// (36 x 4 items of two tiles and 256 rows, D = 64: 31 us with every border where it falls, 19 us with moved ones.)
+// (36 x 4 items of two tiles and 256 rows, D = 64: 31 us with every border where it falls, 19 us with moved ones, 12 today.
+// Prompts and single tokens over up to 3000 keys, 32/8 heads, D = 128: 95 us with these costs, 106 us with a tile of 256 rows
+// counted as two of a few and two tiles for every start.)
 //
 // One launch. Every block scans the requests by itself in shared memory (a few thousand numbers: cheaper than a second
 // launch that waits for the first), then block 0 writes the work list while the others place tokens, one per thread.
@@ -59,7 +60,8 @@ __device__ __forceinline__ T block_exclusive(T v, T* warp_tot, T& total) {
 }
 
 // How far a border may move, by the cost of the item's tiles.
-__device__ __forceinline__ int snap_of(int cost) { return cost == 2 ? 4 : 1; }
+__device__ __forceinline__ int snap_of(int cost) { return cost == kTileCost2 ? 2 * kTileCost2 : kTileCost1; }
+__device__ __forceinline__ int item_cost(int cost) { return cost == kTileCost2 ? kItemCost2 : kItemCost1; }
 
 // Largest index r in [0, n) with a[r] <= x (a ascends, a[0] <= x).
 __device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
@@ -159,7 +161,7 @@ paged_plan_kernel(const PagedPlanDev p) {
     const int i = base + tid;
     int4 a = make_int4(0, 0, 0, 0);
     long long tiles = 0;
-    int cost = 1;
+    int cost = kTileCost1;
     if (i < n_items) {
       const int r = last_not_above(first_item, p.B, i);
       const int t0 = (i - first_item[r]) * p.item_tokens;
@@ -167,10 +169,10 @@ paged_plan_kernel(const PagedPlanDev p) {
       const long long pos0 = context(r) + t0;
       a = make_int4(cu[r] + t0, n, static_cast<int>(min(pos0, static_cast<long long>(INT_MAX / 2))), r);
       tiles = max(1LL, (min(pos0 + n, capacity) + 127) >> 7);
-      cost = 2 * n > p.item_tokens ? 2 : 1;
+      cost = 2 * n > p.item_tokens ? kTileCost2 : kTileCost1;
     }
     long long all;
-    const long long before = carry + block_exclusive(i < n_items ? (tiles + 2) * cost : 0LL, warp_tot, all);
+    const long long before = carry + block_exclusive(i < n_items ? tiles * cost + item_cost(cost) : 0LL, warp_tot, all);
     if (i < n_items) {
       items[2 * i] = a;
       items[2 * i + 1] = make_int4(static_cast<int>(before), static_cast<int>(tiles), cost, 0);
@@ -205,12 +207,12 @@ paged_plan_kernel(const PagedPlanDev p) {
         }
       }
       const int4 item = items[2 * static_cast<long long>(lo) + 1];
-      const int cost = item.z, in = max(0, rem - item.x - 2 * cost), left = item.y * cost - in;
+      const int cost = item.z, in = max(0, rem - item.x - item_cost(cost)), left = item.y * cost - in;
       const int snap = static_cast<int>(min(static_cast<long long>(snap_of(cost)), share >> 1));
       int tile = (in + cost - 1) / cost;
       if (in <= snap && in <= left) tile = 0;
       else if (left <= snap) tile = item.y;
-      start = make_int4(hk, lo, tile, cost == 2);
+      start = make_int4(hk, lo, tile, cost == kTileCost2);
       if (tile >= item.y) start = lo + 1 < n_items ? make_int4(hk, lo + 1, 0, 0) : make_int4(hk + 1, 0, 0, 0);
     }
     reinterpret_cast<int4*>(p.work + kWorkHeader)[c] = start;
