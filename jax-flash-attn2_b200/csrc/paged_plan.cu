@@ -183,7 +183,8 @@ paged_plan_kernel(const PagedPlanDev p) {
   // ---- shares (the items written above are visible to the block behind the barrier)
   __syncthreads();
   const long long per_head = carry, line = per_head * p.heads_kv;
-  const int ctas = static_cast<int>(min(line, static_cast<long long>(p.sms)));
+  // (no more shares than key tiles, about: one without a tile costs the join the look at it)
+  const int ctas = static_cast<int>(min(line / kTileCost1, static_cast<long long>(p.sms)));
   if (tid == 0) {
     p.work[0] = n_items;
     p.work[1] = ctas;

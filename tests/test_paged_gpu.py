@@ -99,7 +99,7 @@ def test_work_list_covers_every_token_once(heads_q, heads_kv):
     work = plan.work.tolist()
     sms = torch.cuda.get_device_properties(0).multi_processor_count
     at = 16 + (4 * (sms + 1) + 7) // 8 * 8
-    assert work[:2] == [len(want), min(sms, before * heads_kv)]
+    assert work[:2] == [len(want), min(sms, before * heads_kv // 2)]
     assert work[at:at + 8 * len(want)] == [x for w in want for x in w]
     # the CTAs' starts go through every tile of every item and head once, in order
     starts = [tuple(work[16 + 4 * c:19 + 4 * c]) for c in range(work[1] + 1)]
