@@ -569,12 +569,23 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   }
 }
 
-// kRows rows of an item at a time, x0, x0 + stride, ...; the parts of CTAs c - 1 .. last that `parts` says are there (bit i:
-// CTA base + i, 32 at a time), kParts of them with their loads under way at once: a part's row comes from L2, and one after
+// Which of the CTAs base .. base + 31 have a part of the item that is cut first at the start of CTA c and reaches to CTA `last`:
+// one without a tile of its own (its start is the next one's) has none, the first one, c - 1, always has.
+__device__ __forceinline__ unsigned paged_parts(const PagedAttnDev& p, int base, int c, int last, int lane) {
+  bool here = base + lane <= last;
+  if (here && base + lane >= c) {
+    const int4 from = paged_start_of(p.work, base + lane), to = paged_start_of(p.work, base + lane + 1);
+    here = from.x != to.x || from.y != to.y || from.z != to.z;
+  }
+  return __ballot_sync(0xffffffffu, here);
+}
+
+// kRows rows of an item at a time, x0, x0 + stride, ...; the parts of CTAs c - 1 .. last that there are (32 CTAs at a time, the
+// first ones known already), kParts of them with their loads under way at once: a part's row comes from L2, and one after
 // the other they would cost its latency each.
 template <int D, bool kBf16, int kRows, int kParts>
 __device__ __forceinline__ void paged_join_rows(const PagedAttnDev& p, int hk, int row0, int rows, int x0, int stride, int c,
-                                                int last, int lane) {
+                                                int last, unsigned first_parts, int lane) {
   constexpr int kVec = D / 32;
   const int row_tile = p.tile_tokens * p.G;
   int row[kRows];                   // inside a part
@@ -589,13 +600,7 @@ __device__ __forceinline__ void paged_join_rows(const PagedAttnDev& p, int hk, i
     for (int e = 0; e < kVec; ++e) acc[k][e] = 0.f;
   }
   for (int base = c - 1; base <= last; base += 32) {
-    // a CTA without a tile of its own (its start is the next one's) has no part; the first one, c - 1, always has
-    bool here = base + lane <= last;
-    if (here && base + lane >= c) {
-      const int4 from = paged_start_of(p.work, base + lane), to = paged_start_of(p.work, base + lane + 1);
-      here = from.x != to.x || from.y != to.y || from.z != to.z;
-    }
-    unsigned parts = __ballot_sync(0xffffffffu, here);
+    unsigned parts = base == c - 1 ? first_parts : paged_parts(p, base, c, last, lane);
     while (parts) {
       float lse[kParts][kRows], v[kParts][kRows][kVec];
 #pragma unroll
@@ -682,15 +687,16 @@ paged_combine_kernel(const PagedAttnDev p) {
       }
     }
   }
+  const unsigned parts = first_inside ? paged_parts(p, c - 1, c, last, lane) : 0u;
   // (every block waits, so that this kernel never ends before the main one)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!first_inside) return;
   const int rows = a.y * p.G, stride = 8 * gridDim.y;
   int x = (threadIdx.x >> 5) + 8 * blockIdx.y;
   if (rows <= stride) {
-    if (x < rows) paged_join_rows<D, kBf16, 1, 8>(p, at.x, a.x, rows, x, stride, c, last, lane);
+    if (x < rows) paged_join_rows<D, kBf16, 1, 8>(p, at.x, a.x, rows, x, stride, c, last, parts, lane);
   } else {
-    for (; x < rows; x += 4 * stride) paged_join_rows<D, kBf16, 4, 2>(p, at.x, a.x, rows, x, stride, c, last, lane);
+    for (; x < rows; x += 4 * stride) paged_join_rows<D, kBf16, 4, 2>(p, at.x, a.x, rows, x, stride, c, last, parts, lane);
   }
 }
 
