@@ -288,7 +288,7 @@ int bwd_parts(const fa2_problem& p, const HeadDim& hd) {
   const int64_t steps = (static_cast<int64_t>(p.seqlen_q) + 127) / 128 * group;
   return steps - steps / parts >= 2 ? static_cast<int>(parts) : 1;
 }
-BwdWorkspace bwd_workspace(const fa2_problem& p) {
+BwdWorkspace bwd_workspace(const fa2_problem& p, bool scored = false) {
   BwdWorkspace w;
   w.sq_pad = (p.seqlen_q + 127) / 128 * 128;
   const size_t rows = static_cast<size_t>(p.batch) * p.heads_q * w.sq_pad;
@@ -304,7 +304,7 @@ BwdWorkspace bwd_workspace(const fa2_problem& p) {
   // counters for the bit-reproducible mode: one per 128-row dQ tile, at head dim 256 one per
   // 64 rows and half of the head dim
   w.total = w.order_off + align_up(rows / 128 * (hd.padded <= 128 ? 1 : 4) * sizeof(int), 256);
-  w.parts = bwd_parts(p, hd);
+  w.parts = scored ? bwd_parts(p, hd) : 1;
   w.parts_off = w.total;
   const size_t kv_rows = static_cast<size_t>(p.batch) * p.heads_kv * ((static_cast<size_t>(p.seqlen_k) + 127) / 128 * 128);
   w.parts_total = w.total + (w.parts > 1 ? 2 * w.parts * kv_rows * hd.padded * sizeof(float) : 0);
@@ -549,7 +549,7 @@ int fa2_scored_fwd(const fa2_fwd_params* a, const fa2_score_mod* mod, void* cuda
 
 size_t fa2_scored_bwd_workspace_bytes(const fa2_problem* problem) {
   if (!problem || check_problem(*problem)) return 0;
-  return bwd_workspace(*problem).parts_total;
+  return bwd_workspace(*problem, true).parts_total;
 }
 
 int fa2_scored_bwd(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_stream) {
@@ -1005,7 +1005,7 @@ int bwd_impl(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_strea
     return fail(FA2_ERR_INVALID_ARG, "q, k, v, o, d_o, lse, dq, dk and dv must be non-null");
   if (a->lse_stride_h < p.seqlen_q || a->lse_stride_b < 0)
     return fail(FA2_ERR_INVALID_ARG, "lse_stride_h must be at least seqlen_q");
-  const BwdWorkspace w = bwd_workspace(p);
+  const BwdWorkspace w = bwd_workspace(p, mod != nullptr);
   if (!a->workspace || a->workspace_bytes < w.total)
     return fail(FA2_ERR_WORKSPACE, "workspace must hold %zu bytes", w.total);
   if (reinterpret_cast<uintptr_t>(a->workspace) & (kWorkspaceAlign - 1))
@@ -1119,7 +1119,7 @@ int bwd_impl(const fa2_bwd_params* a, const fa2_score_mod* mod, void* cuda_strea
   L.d_o = a->d_o; L.do_strides[0] = a->do_strides.b; L.do_strides[1] = a->do_strides.s; L.do_strides[2] = a->do_strides.h;
   L.dq = a->dq; L.dq_strides[0] = a->dq_strides.b; L.dq_strides[1] = a->dq_strides.s; L.dq_strides[2] = a->dq_strides.h;
   L.parts = 1;
-  if (mod && w.parts > 1 && a->workspace_bytes >= w.parts_total) {
+  if (w.parts > 1 && a->workspace_bytes >= w.parts_total) {
     L.parts = w.parts;
     kp.part_kv = reinterpret_cast<float*>(ws + w.parts_off);
     L.dk = a->dk; L.dk_strides[0] = a->dk_strides.b; L.dk_strides[1] = a->dk_strides.s; L.dk_strides[2] = a->dk_strides.h;
