@@ -22,7 +22,7 @@ BINDING_PATH = os.path.join(HERE, "jax_flash_attn2", "_fa2_native.so")
 SOURCES = ["api.cu", "fwd_sm100.cu", "fwd256_sm100.cu", "fwd_combine.cu", "bwd_sm100.cu", "bwd256_sm100.cu",
            "fwd_scored64_sm100.cu", "fwd_scored128_sm100.cu", "fwd_scored256_sm100.cu",
            "bwd_scored64_sm100.cu", "bwd_scored128_sm100.cu", "bwd_scored256_sm100.cu", "document_layout.cu",
-           "paged_plan.cu", "paged64_sm100.cu", "paged128_sm100.cu"]
+           "paged_plan.cu", "paged64_sm100.cu", "paged128_sm100.cu", "paged128_rows_sm100.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -799,6 +799,15 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
     const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(tile_tokens), 1, 1};
     if ((rc = encode_map(&L.tmQ, a->q, bf16, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, "q"))) return rc;
   }
+  // Two column blocks in one box: the places of a page count as groups of 8, and one dimension serves for two where pages lie
+  // one behind the other (groups of all pages) or the heads of all pages do.
+  const int64_t page_groups = a->page_size / 8, all_groups = page_groups * (a->pages + INT64_C(1)),
+                all_heads = a->heads_kv * (a->pages + INT64_C(1));
+  const auto pages_in_line = [&](const fa2_paged_cache& c) { return c.stride_page == c.stride_slot * a->page_size; };
+  const auto heads_in_line = [&](const fa2_paged_cache& c) { return c.stride_page == c.stride_head * a->heads_kv; };
+  const bool by_groups = all_groups <= INT_MAX && pages_in_line(a->k_cache) && pages_in_line(a->v_cache);
+  const bool by_heads = !by_groups && all_heads <= INT_MAX && heads_in_line(a->k_cache) && heads_in_line(a->v_cache);
+  const bool whole_rows = hd.padded == 128 && (by_groups || by_heads);
   for (int x = 0; x < 2; ++x) {
     // (columns, places in a page, column blocks, heads, pages): a box is a piece of a page of at most 128 rows
     const fa2_paged_cache& c = x ? a->v_cache : a->k_cache;
@@ -811,6 +820,16 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
     // before another CTA comes there (16 decodes over 16000 keys, 16/8 heads, D = 64, pages of 64: 138 us, 121 with 128).
     const CUtensorMapL2promotion promotion =
         hd.padded == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+    if (whole_rows) {
+      // (columns, 8 places, column blocks, groups of 8 places, heads)
+      const cuuint64_t dims_w[5] = {static_cast<cuuint64_t>(hd.blk), 8, static_cast<cuuint64_t>(hd.nblk),
+                                    static_cast<cuuint64_t>(by_groups ? page_groups * a->pages : page_groups),
+                                    static_cast<cuuint64_t>(by_groups ? a->heads_kv : static_cast<int64_t>(a->heads_kv) * a->pages)};
+      const cuuint64_t st_w[4] = {bytes(c.stride_slot), bytes(hd.blk), bytes(c.stride_slot * 8), bytes(c.stride_head)};
+      const cuuint32_t box_w[5] = {64, 8, 2, static_cast<cuuint32_t>(std::min(a->page_size, 128) / 8), 1};
+      if ((rc = encode_map(x ? &L.tmV : &L.tmK, c.ptr, bf16, dims_w, st_w, box_w, promotion, x ? "v_cache" : "k_cache"))) return rc;
+      continue;
+    }
     if ((rc = encode_map(x ? &L.tmV : &L.tmK, c.ptr, bf16, dims, st, box, promotion, x ? "v_cache" : "k_cache"))) return rc;
   }
   PagedAttnDev& d = L.p;
@@ -823,6 +842,8 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
   d.table_width = a->table_width;
   d.page_shift = shift;
   d.num_pages = a->pages;
+  d.page_groups = by_groups ? static_cast<int>(page_groups) : 0;
+  d.page_heads = by_groups ? 0 : a->heads_kv;
   d.scale_log2 = static_cast<float>(a->softmax_scale * 1.4426950408889634);
   L.mod = 0;
   if (a->softcap > 0.f) {
@@ -841,6 +862,7 @@ int fa2_paged_attention(const fa2_paged_attention_params* a, void* cuda_stream) 
   d.part_lse = d.part_o + static_cast<size_t>(2) * sm_count() * 256 * hd.padded;
   d.status = status_word;
   L.head_dim = hd.padded;
+  L.whole_rows = whole_rows;
   L.bf16 = bf16;
   const cudaError_t e = launch_paged_attention(L, static_cast<cudaStream_t>(cuda_stream));
   if (e != cudaSuccess) return fail(FA2_ERR_CUDA, "paged attention launch failed: %s", cudaGetErrorString(e));

@@ -62,6 +62,7 @@ struct PagedAttnDev {
   const int* block_table;
   long long table_stride;
   int table_width, page_shift, num_pages;
+  int page_groups, page_heads;   // whole_rows: what a page adds to a box's fourth and fifth coordinate
   float scale_log2, cap2, arg2;
   const float* slopes;       // [Hq] or null
   uint16_t* out;
@@ -76,6 +77,7 @@ struct PagedAttnLaunch {
   CUtensorMap tmQ, tmK, tmV;
   PagedAttnDev p;
   int head_dim;              // 64 or 128
+  bool whole_rows;           // (head dim 128) a box of K or V brings all columns of its keys
   bool bf16;
   int mod;                   // kModCap | kModSlope
 };

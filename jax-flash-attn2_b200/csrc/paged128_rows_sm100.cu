@@ -1,0 +1,10 @@
+// Attention over a paged cache, head dims up to 128 (paged_attention.cuh), a box of the cache for all columns of its keys.
+#include "paged_attention.cuh"
+
+namespace fa2 {
+
+cudaError_t launch_paged_attention128_rows(const PagedAttnLaunch& a, cudaStream_t stream) {
+  return launch_paged_dim<128, true>(a, stream);
+}
+
+}  // namespace fa2

@@ -20,7 +20,9 @@
 // 137 us with two; the cache alone is 646 MB, 98 us at the measured copy bandwidth.
 //
 // Keys. Pages hold 2^s tokens; a 128-key tile takes 128 / 2^s pieces of a page each (one if pages are larger), every piece
-// and 64-column block one TMA box, issued by a lane of its own. Pages outside the request or the pool are fetched from
+// one TMA box, issued by a lane of its own, or one per 64-column block where the cache's strides leave no dimension of a
+// tensor map for the blocks (64 tokens over 9856 keys in pages of 16, 32/8 heads, D = 128: 414 us, 469 with a box per block, which
+// is 2 KB; pages of 32 and more: no difference). Pages outside the request or the pool are fetched from
 // an index behind the pool, which the TMA unit fills with zeros. Keys behind the last visible one in its page hold whatever
 // was in memory: their scores are masked, and a spare warp zeroes their V rows, since 0 * NaN is NaN.
 //
@@ -164,7 +166,8 @@ __device__ __forceinline__ bool paged_next(const PagedAttnDev& p, PagedWalk& w, 
 
 }  // namespace
 
-template <int D, bool kBf16, int kMod>
+// kWhole: a box brings all columns of its keys.
+template <int D, bool kBf16, int kMod, bool kWhole>
 __global__ void __launch_bounds__(kPagedThreads, 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                        const __grid_constant__ CUtensorMap tmV, const PagedAttnDev p) {
@@ -187,6 +190,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_gen + L::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + L::kMiscOff + 4);
   constexpr int kBlks = D / 64;
+  // a K or V tile: groups of 8 keys, 1 KiB per column block; all groups of a block together, or (kWhole) all blocks of a group
+  constexpr int group_stride = kWhole ? kBlks * 1024 : 1024, blk_stride = kWhole ? 1024 : L::kBlock;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 9 && lane == 0) {
@@ -252,7 +257,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       uint8_t* v = smem_gen + L::kKVOff + slot * L::kKVTileBytes;
       for (int x = lane; x < (end - tail) * 8 * kBlks; x += 32) {
         const int blk = x / ((end - tail) * 8), y = x - blk * ((end - tail) * 8);
-        *reinterpret_cast<uint4*>(v + blk * L::kBlock + tail * 128 + y * 16) = make_uint4(0u, 0u, 0u, 0u);
+        const int row = tail + (y >> 3);
+        *reinterpret_cast<uint4*>(v + blk * blk_stride + (row >> 3) * group_stride + (row & 7) * 128 + (y & 7) * 16) =
+            make_uint4(0u, 0u, 0u, 0u);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -266,8 +273,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     PagedSeg s;
     const int piece_rows = min(128, 1 << p.page_shift), pieces = 128 / piece_rows;
     const int my_piece = lane % pieces, my_blk = lane / pieces;    // this lane's box of a K or V tile
-    const bool issues = my_blk < kBlks;
-    const uint32_t box_dst = my_blk * L::kBlock + my_piece * piece_rows * 128;
+    const bool issues = my_blk < (kWhole ? 1 : kBlks);
+    const uint32_t box_dst = my_blk * L::kBlock + my_piece * piece_rows * (kWhole ? 128 * kBlks : 128);
     const int page_mask = (1 << p.page_shift) - 1;
     const uint32_t q_bytes = static_cast<uint32_t>(p.tile_tokens * p.G) * 128u * kBlks;
     for (; ok && paged_next(p, w, s); ++seg_idx) {
@@ -299,9 +306,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (!ok) return;
         if (lane == 0) mbar_arrive_expect_tx(bar_kv_full(slot), L::kKVTileBytes);
         __syncwarp();
-        if (issues)
-          tma_load_5d(sKV + slot * L::kKVTileBytes + box_dst, tm, bar_kv_full(slot), 0,
-                      (j * 128 + my_piece * piece_rows) & page_mask, my_blk, s.hk, page);
+        const int place = (j * 128 + my_piece * piece_rows) & page_mask;
+        if (kWhole && issues)
+          tma_load_5d(sKV + slot * L::kKVTileBytes + box_dst, tm, bar_kv_full(slot), 0, 0, 0,
+                      page * p.page_groups + (place >> 3), page * p.page_heads + s.hk);
+        else if (issues)
+          tma_load_5d(sKV + slot * L::kKVTileBytes + box_dst, tm, bar_kv_full(slot), 0, place, my_blk, s.hk, page);
         ++kv_count;
       };
       // in the order in which the MMA warp uses them (see there); pages are looked up two tiles ahead
@@ -323,15 +333,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     constexpr uint32_t idesc_o = make_idesc(kBf16, kBM, D, false, true);
     bool ok = true;
     const uint64_t dQ0 = make_sdesc(sQ, 16, 1024);
-    const uint64_t dKV_k0 = make_sdesc(sKV, 16, 1024);               // K tile, K-major
-    const uint64_t dKV_mn0 = make_sdesc(sKV, L::kBlock, 1024);       // V tile, MN-major
+    const uint64_t dKV_k0 = make_sdesc(sKV, 16, group_stride);               // K tile, K-major
+    const uint64_t dKV_mn0 = make_sdesc(sKV, blk_stride, group_stride);      // V tile, MN-major
     auto issue_s = [&](int t, int slot, int q_tile) {
       const uint64_t a0 = sdesc_advance(dQ0, q_tile * L::kQTileBytes);
       const uint64_t b0 = sdesc_advance(dKV_k0, slot * L::kKVTileBytes);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (k >> 2) * L::kBlock + (k & 3) * 32;
-        mma_ss_e(tmem_base + kColS + t * kBN, sdesc_advance(a0, off), sdesc_advance(b0, off), idesc_s, k > 0 ? 1u : 0u);
+        const uint32_t off = (k & 3) * 32;
+        mma_ss_e(tmem_base + kColS + t * kBN, sdesc_advance(a0, (k >> 2) * L::kBlock + off),
+                 sdesc_advance(b0, (k >> 2) * blk_stride + off), idesc_s, k > 0 ? 1u : 0u);
       }
       mma_commit_e(bar_s_full(t));
     };
@@ -339,7 +350,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const uint64_t b0 = sdesc_advance(dKV_mn0, slot * L::kKVTileBytes);
 #pragma unroll
       for (int k = hh * (kPCols / 16); k < (hh + 1) * (kPCols / 16); ++k)
-        mma_ts_e(tmem_base + kColO + t * D, tmem_base + kColS + t * kBN + k * 8, sdesc_advance(b0, k * 2048), idesc_o,
+        mma_ts_e(tmem_base + kColO + t * D, tmem_base + kColS + t * kBN + k * 8, sdesc_advance(b0, k * 2 * group_stride), idesc_o,
                  (first && k == 0) ? 0u : 1u);
     };
     uint32_t kv_count = 0, seg_idx = 0;
@@ -700,10 +711,10 @@ paged_combine_kernel(const PagedAttnDev p) {
   }
 }
 
-template <int D, bool kBf16, int kMod>
+template <int D, bool kBf16, int kMod, bool kWhole>
 static cudaError_t launch_paged_one(const PagedAttnLaunch& a, cudaStream_t stream) {
   using L = PagedSmem<D>;
-  auto kern = paged_attention_kernel<D, kBf16, kMod>;
+  auto kern = paged_attention_kernel<D, kBf16, kMod, kWhole>;
   static bool smem_opted_in[64] = {};
   cudaError_t e = opt_in_dynamic_smem(kern, L::kDynamicBytes, smem_opted_in);
   if (e != cudaSuccess) return e;
@@ -724,17 +735,17 @@ static cudaError_t launch_paged_one(const PagedAttnLaunch& a, cudaStream_t strea
   return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, kBf16>, a.p);
 }
 
-template <int D>
+template <int D, bool kWhole>
 static cudaError_t launch_paged_dim(const PagedAttnLaunch& a, cudaStream_t stream) {
   switch ((a.bf16 ? 4 : 0) | a.mod) {
-    case 0: return launch_paged_one<D, false, 0>(a, stream);
-    case 1: return launch_paged_one<D, false, 1>(a, stream);
-    case 2: return launch_paged_one<D, false, 2>(a, stream);
-    case 3: return launch_paged_one<D, false, 3>(a, stream);
-    case 4: return launch_paged_one<D, true, 0>(a, stream);
-    case 5: return launch_paged_one<D, true, 1>(a, stream);
-    case 6: return launch_paged_one<D, true, 2>(a, stream);
-    default: return launch_paged_one<D, true, 3>(a, stream);
+    case 0: return launch_paged_one<D, false, 0, kWhole>(a, stream);
+    case 1: return launch_paged_one<D, false, 1, kWhole>(a, stream);
+    case 2: return launch_paged_one<D, false, 2, kWhole>(a, stream);
+    case 3: return launch_paged_one<D, false, 3, kWhole>(a, stream);
+    case 4: return launch_paged_one<D, true, 0, kWhole>(a, stream);
+    case 5: return launch_paged_one<D, true, 1, kWhole>(a, stream);
+    case 6: return launch_paged_one<D, true, 2, kWhole>(a, stream);
+    default: return launch_paged_one<D, true, 3, kWhole>(a, stream);
   }
 }
 

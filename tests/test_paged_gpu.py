@@ -474,3 +474,23 @@ def test_a_pool_of_more_than_2_31_elements():
         outs.append(J.paged_attention(q, *caches, plan))
     assert torch.equal(outs[0], outs[1]) and torch.equal(small[0], large[0][-used:]) and torch.equal(small[1], large[1][-used:])
     assert torch.isfinite(outs[0].float()).all() and J.device_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("page", [8, 16, 64, 256])
+def test_every_layout_of_the_cache_gives_the_same_bits(D, page):
+    import jax_flash_attn2 as J
+    g = torch.Generator().manual_seed(page + D)
+    Hq, Hkv, context, new = 6, 3, [300, 0, 41, 700], [1, 130, 7, 1]
+    table, free, pages = make_step(context, new, page)
+    k, v = (torch.randn(pages, page, Hkv, D, generator=g).to(BF16).cuda() for _ in range(2))
+    q = torch.randn(sum(new), Hq, D, generator=g).to(BF16).cuda()
+    plan = J.paged_step_plan(dev_int(context), dev_int(new), dev_int(table), dev_int(free), page_size=page, num_tokens=sum(new),
+                             heads_q=Hq, heads_kv=Hkv)
+    both = torch.stack([k, v], 1)                                          # [pages, 2, page, Hkv, D]
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v)]
+    wide = [torch.nn.functional.pad(x, (0, 8)).contiguous()[..., :D] for x in (k, v)]      # rows of D + 8
+    layouts = [(k, v), (both[:, 0], both[:, 1]), heads_first, (k, heads_first[1]), wide]
+    assert heads_first[0].stride(1) == D and both[:, 0].stride(0) == 2 * page * Hkv * D
+    outs = [J.paged_attention(q, *x, plan) for x in layouts]
+    assert torch.isfinite(outs[0].float()).all() and all(torch.equal(x, outs[0]) for x in outs) and J.device_status() == 0
