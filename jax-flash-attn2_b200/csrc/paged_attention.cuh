@@ -17,7 +17,7 @@
 // tile, not by its work. It runs as two chains: the second warpgroup takes the odd key tiles of the same rows, with its own
 // maximum, sum and accumulator, and the first one joins the two accumulators when it writes the rows, straight from tensor
 // memory (the rows lie on the same lanes). 64 decodes over 128 .. 16384 keys (32/8 heads, D = 128): 161 us with one chain,
-// 137 us with two; the cache alone is 646 MB, 98 us at the measured copy bandwidth.
+// 137 us with two (124 today); the cache alone is 646 MB, 98 us at the measured copy bandwidth.
 //
 // Keys. Pages hold 2^s tokens; a 128-key tile takes 128 / 2^s pieces of a page each (one if pages are larger), every piece
 // one TMA box, issued by a lane of its own, or one per 64-column block where the cache's strides leave no dimension of a
